@@ -1,0 +1,584 @@
+// Causal grouped-query attention over the 8-bit cache (layout: kv8.cuh), compiled for one head size:
+// -DFE_HEAD_DIM=<multiple of 16, 16..256>.
+//
+// A query at position i of a sequence sees the keys j <= i, or with a window those of the last `window`
+// positions and the first `keep_first`.  With cached key code c_j, value code d_j and their scales 2^a_j, 2^b_j:
+//
+//   t_j = scale * log2(e) * (q . c_j) 2^a_j            out = sum_j 2^(t_j) 2^b_j d_j / sum_j 2^(t_j)
+//
+// Neither matrix is ever scaled element by element: 2^a_j is a factor of a finished score, and 2^b_j joins the
+// exponent, u_j = t_j + b_j.  The running maximum M is that of u_j, the largest contribution to the output, so
+// the weights 2^(u_j - M) of the value product lie in [0, 1] whatever the scales are, and the codes go into the
+// tensor cores as the half-precision numbers they exactly are (one conversion instruction for two codes).  The
+// denominator sums 2^(t_j - M) = 2^(u_j - M) 2^(-b_j) in 32 bits.  Weights are rounded to half precision (11
+// bits; what is below 2^-25 of the largest contribution vanishes).  A query row is scaled by a power of two so
+// that its largest element lies in [2^14, 2^15): bfloat16's 8 bits stay whole down to 2^-31 of that.
+//
+// Upstream's counterparts read pages of the model's type: the eager attention of
+// src/forge_engine/qwen3.py:187-206 and the decode kernel of src/forge_engine/kernels/cuda_paged.py:276-347.
+#include <cuda_fp16.h>
+
+#include "kv8.cuh"
+
+#ifndef FE_HEAD_DIM
+#error "compile with -DFE_HEAD_DIM=<head size>"
+#endif
+#define CAT_(a, b) a##b
+#define CAT(a, b) CAT_(a, b)
+#define SYM(name) CAT(name, FE_HEAD_DIM)
+
+namespace {
+
+constexpr int D = FE_HEAD_DIM;
+static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 up to 256");
+constexpr int CHUNKS = D / 16;          // 16-byte pieces of a cached vector
+constexpr int KEYS = 64;                // keys of a tile
+constexpr int ROWS = 16;                // rows a warp takes: the m of one mma
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int STAGES = D <= 128 ? 4 : 3;
+constexpr int MATRIX = KEYS * D;        // bytes of one matrix of a stage
+constexpr int STAGE = 2 * MATRIX + 2 * KEYS;
+constexpr size_t MMA_SMEM_RING = (size_t)STAGES * STAGE;
+constexpr size_t MMA_SMEM_JOIN = (size_t)WARPS * ROWS * (D + 2) * sizeof(float);
+constexpr size_t MMA_SMEM = MMA_SMEM_RING > MMA_SMEM_JOIN ? MMA_SMEM_RING : MMA_SMEM_JOIN;
+
+struct Kv8Attention {
+  const bf16* q;
+  long long q_stride;
+  bf16* out;               // [tokens, nkv * groups * D]
+  const unsigned char *k, *v, *ks, *vs;
+  const int* block_table;
+  int max_pages, page_size, page_shift, num_pages, nkv, groups;
+  const int* cu_tokens;    // [entries + 1]
+  const int* starts;       // [entries]
+  int total_tokens, window, keep_first;
+  float scale_log2;
+  int* status;
+  int row_lo, row_hi;      // entries with row_lo < rows <= row_hi
+  int span, spans;         // a block takes `span` key tiles of a unit; the grid holds `spans` of them
+  int units;               // row tiles of the longest entry
+  float* ws;               // [entries, nkv, units, spans, rows of a unit, D + 2]: sums, then M and l
+};
+
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0));
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 4 : 0));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+__device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// The key tiles (of TILE keys) that the rows [row0, row0 + n) of an entry see: first the tiles that hold kept
+// first tokens and lie before the window, then the window's.
+template <int TILE>
+struct Walk {
+  int pos_first, pos_last, key_lo, key_end, kept, first, count;
+  __device__ __forceinline__ Walk(const Kv8Attention& p, int start, int row0, int rows_end) {
+    pos_first = start + row0 / p.groups;
+    pos_last = start + (rows_end - 1) / p.groups;
+    key_lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
+    key_end = pos_last + 1;
+    first = key_lo / TILE;
+    kept = p.window > 0 ? min((p.keep_first + TILE - 1) / TILE, first) : 0;
+    count = kept + (key_end + TILE - 1) / TILE - first;
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < kept ? i : first + i - kept; }
+};
+
+// Pieces of a unit of `count` key tiles; where the grid holds fewer than its spans give, the last takes the rest.
+__device__ __forceinline__ int pieces_of(const Kv8Attention& p, int count) { return min(p.spans, (count + p.span - 1) / p.span); }
+
+// Tokens of an entry, held to the tensors the call brought.
+struct Entry {
+  int tok0, n_new, start;
+  __device__ __forceinline__ Entry(const Kv8Attention& p, int entry) {
+    tok0 = p.cu_tokens[entry];
+    n_new = p.cu_tokens[entry + 1] - tok0;
+    start = p.starts[entry];
+    if (tok0 < 0 || n_new < 0 || tok0 > p.total_tokens - n_new || start < 0 || start > 0x7fff0000 - n_new) {
+      if (threadIdx.x == 0) atomicOr(p.status, FE_STATUS_BAD_POSITION);
+      n_new = 0;
+    }
+  }
+};
+
+// Row (page, head, slot) of a key, or -1 where its page is missing (flagged if some row must see it).
+__device__ __forceinline__ long long key_row(const Kv8Attention& p, const int* table, int kvh, int key, bool needed) {
+  const int logical = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+  const int page = logical < p.max_pages ? table[logical] : -1;
+  if (page < 0 || page >= p.num_pages) {
+    if (needed) atomicOr(p.status, FE_STATUS_BAD_PAGE);
+    return -1;
+  }
+  return ((long long)page * p.nkv + kvh) * p.page_size + (key - logical * p.page_size);
+}
+
+// Where 16-byte piece c of row r lies.  Keys are read 8 rows x 4 pieces at a time (rows two by two in a phase
+// of a shared-memory read), values the rows 2t, 2t + 1, 2t + 8, 2t + 9 x pieces of 8 lanes: each matrix has the
+// exchange of pieces that keeps its reads apart.  Head sizes without a whole power of two of pieces take none.
+__device__ __forceinline__ int key_piece(int r, int c) { return D % 128 == 0 ? c ^ ((r & 1) << 2) : c; }
+__device__ __forceinline__ int value_piece(int r, int c) {
+  return D % 128 == 0 ? c ^ (((r >> 1) & 3) << 1) : D % 64 == 0 ? c ^ ((r >> 1) & 3) : c;
+}
+
+// Stage the keys [key0, key0 + 64) of one kv head, their values and both scales.  What lies at or past key_end
+// is zero.
+__device__ __forceinline__ void load_tile(unsigned char* stage, const Kv8Attention& p, const int* table, int kvh, int key0,
+                                          int key_lo, int key_end, int tid) {
+  unsigned char* kd = stage;
+  unsigned char* vd = stage + MATRIX;
+  unsigned char* sd = stage + 2 * MATRIX;
+#pragma unroll
+  for (int u = tid; u < KEYS * CHUNKS; u += THREADS) {
+    const int row = u / CHUNKS, c = u - row * CHUNKS, key = key0 + row;
+    long long at = key < key_end ? key_row(p, table, kvh, key, c == 0 && (key >= key_lo || key < p.keep_first)) : -1;
+    const bool valid = at >= 0;
+    if (!valid) at = 0;
+    cp_async16(kd + row * D + key_piece(row, c) * 16, p.k + at * D + c * 16, valid);
+    cp_async16(vd + row * D + value_piece(row, c) * 16, p.v + at * D + c * 16, valid);
+  }
+  if (p.page_size % 4 == 0) {          // four neighbouring scales lie in one word
+    if (tid < 2 * (KEYS / 4)) {
+      const int row = (tid % (KEYS / 4)) * 4, m = tid / (KEYS / 4), key = key0 + row;
+      long long at = key < key_end ? key_row(p, table, kvh, key, false) : -1;
+      const bool valid = at >= 0;
+      cp_async4(sd + m * KEYS + row, (m ? p.vs : p.ks) + (valid ? at : 0), valid);
+    }
+  } else {
+    const int row = tid % KEYS, m = tid / KEYS, key = key0 + row;
+    const long long at = key < key_end ? key_row(p, table, kvh, key, false) : -1;
+    sd[m * KEYS + row] = at >= 0 ? (m ? p.vs : p.ks)[at] : 0;
+  }
+}
+
+// The queries of a warp's 16 rows as the A operand.  The order of the contraction is free as long as both
+// operands keep it: in every stretch of 64 elements lane t of a quad holds elements 16 t .. 16 t + 15, which it
+// reads of a key as one 16-byte piece; stretches of 32 and 16 at the end go by 8 and 4 elements.
+struct Queries {
+  unsigned a[D / 16][4];
+  float factor[2];                 // what a product of row g / g + 8 is multiplied by to be a score in log2 units
+
+  static __device__ __forceinline__ int element(int step, int t) {      // first of the lane's four elements of a k step
+    constexpr int whole = D / 64 * 4;
+    if (step < whole) return (step >> 2) * 64 + 16 * t + 4 * (step & 3);
+    int base = D / 64 * 64, s = step - whole;
+    if (D & 32) {
+      if (s < 2) return base + 8 * t + 4 * s;
+      base += 32;
+    }
+    return base + 4 * t;
+  }
+
+  __device__ __forceinline__ void load(const Kv8Attention& p, const Entry& e, int kvh, int row0, int rows_end, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + (lane >> 2) + 8 * h;
+      float x[D / 4];
+      unsigned big = 0u;
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+      if (row < rows_end) {
+        const int token = row / p.groups, g = row - token * p.groups;
+        const bf16* src = p.q + (size_t)(e.tok0 + token) * p.q_stride + (size_t)(kvh * p.groups + g) * D;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) load4(src + element(s, t), x + 4 * s);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      int e2 = (int)(big >> 23) - 127 - 14;                      // 2^e2 is taken out of the row
+      e2 = big == 0u || big >= 0x7f800000u ? 0 : max(e2, -100);
+      const float down = __int_as_float((127 - e2) << 23);
+      factor[h] = p.scale_log2 * __int_as_float((127 + e2) << 23);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        a[s][h] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
+        a[s][h + 2] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
+      }
+    }
+  }
+};
+
+// Running maximum, sum and value sums of a warp's 16 rows; lane (g, t) holds rows g and g + 8.  Value columns
+// are taken in stretches of 128, 64, 32 and 16: in one of 8 W columns lane g of the B operand holds columns
+// W g .. W g + W - 1, which are one read of W bytes of a value, and W products cover the stretch.
+struct Sums {
+  float m[2], l[2];
+  float o[D / 8][4];
+  __device__ __forceinline__ void clear() {
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f; }
+  }
+};
+
+template <int W> struct Piece;
+template <> struct Piece<16> { typedef uint4 type; };
+template <> struct Piece<8> { typedef uint2 type; };
+template <> struct Piece<4> { typedef unsigned type; };
+template <> struct Piece<2> { typedef unsigned short type; };
+
+// Value columns [BASE, BASE + 8 W): o += weights x values, 16 keys.
+template <int BASE, int W>
+__device__ __forceinline__ void value_stretch(const unsigned char* vs, int k0, const unsigned (&a)[4], float (&o)[D / 8][4], int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  constexpr int WORDS = W < 4 ? 1 : W / 4;
+  unsigned w[4][WORDS];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = k0 + 2 * t + (i & 1) + 8 * (i >> 1), byte = BASE + W * g;
+    const typename Piece<W>::type x =
+        *reinterpret_cast<const typename Piece<W>::type*>(vs + row * D + value_piece(row, byte >> 4) * 16 + (byte & 15));
+    if constexpr (W == 16) { w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w; }
+    else if constexpr (W == 8) { w[i][0] = x.x; w[i][1] = x.y; }
+    else w[i][0] = x;
+  }
+#pragma unroll
+  for (int c = 0; c < WORDS; ++c) {
+    // bytes of two rows side by side: (row 2t column j, row 2t + 1 column j), ...
+    const unsigned lo0 = __byte_perm(w[0][c], w[1][c], 0x5140), lo1 = __byte_perm(w[0][c], w[1][c], 0x7362);
+    const unsigned hi0 = __byte_perm(w[2][c], w[3][c], 0x5140), hi1 = __byte_perm(w[2][c], w[3][c], 0x7362);
+    constexpr int N0 = BASE / 8;
+    mma_f16(o[N0 + 4 * c], a, kv8_half2((unsigned short)lo0), kv8_half2((unsigned short)hi0));
+    mma_f16(o[N0 + 4 * c + 1], a, kv8_half2((unsigned short)(lo0 >> 16)), kv8_half2((unsigned short)(hi0 >> 16)));
+    if constexpr (W > 2) {
+      mma_f16(o[N0 + 4 * c + 2], a, kv8_half2((unsigned short)lo1), kv8_half2((unsigned short)hi1));
+      mma_f16(o[N0 + 4 * c + 3], a, kv8_half2((unsigned short)(lo1 >> 16)), kv8_half2((unsigned short)(hi1 >> 16)));
+    }
+  }
+}
+
+// Column of element (n-tile, c) of Sums::o for quad lane t: n-tile BASE/8 + j holds columns W (2 t + c) + j.
+__device__ __forceinline__ int value_column(int n, int c, int t) {
+  int base = 0, left = D;
+  if (n * 8 < D / 128 * 128) { base = n / 16 * 128; return base + 16 * (2 * t + c) + (n & 15); }
+  base = D / 128 * 128; left = D - base;
+  if (left & 64) { if (n * 8 < base + 64) return base + 8 * (2 * t + c) + (n * 8 - base) / 8; base += 64; }
+  if (left & 32) { if (n * 8 < base + 32) return base + 4 * (2 * t + c) + (n * 8 - base) / 8; base += 32; }
+  return base + 2 * (2 * t + c) + (n * 8 - base) / 8;
+}
+
+// 16 keys (k0 .. k0 + 15 of the staged tile, positions from key0 on) against a warp's 16 rows.
+__device__ __forceinline__ void step16(const Queries& q, const unsigned char* stage, int k0, int key0, const Kv8Attention& p,
+                                       bool clear, int pos_a, int pos_b, Sums& s, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  const unsigned char* ks = stage;
+  const unsigned char* scales = stage + 2 * MATRIX;
+  float c[2][4];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+    const int row = k0 + 8 * n + g;
+    unsigned w[D / 16];
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b) {
+      const uint4 x = *reinterpret_cast<const uint4*>(ks + row * D + key_piece(row, 4 * b + t) * 16);
+      w[4 * b] = x.x; w[4 * b + 1] = x.y; w[4 * b + 2] = x.z; w[4 * b + 3] = x.w;
+    }
+    if constexpr ((D & 32) != 0) {
+      const uint2 x = *reinterpret_cast<const uint2*>(ks + row * D + D / 64 * 64 + 8 * t);
+      w[D / 64 * 4] = x.x; w[D / 64 * 4 + 1] = x.y;
+    }
+    if constexpr ((D & 16) != 0) w[D / 16 - 1] = *reinterpret_cast<const unsigned*>(ks + row * D + D - 16 + 4 * t);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      mma_f16(c[n], q.a[i], kv8_half2((unsigned short)w[i]), kv8_half2((unsigned short)(w[i] >> 16)));
+  }
+  // keys k0 + 8 n + 2 t + i: factor of the score, exponent and reciprocal scale of the value
+  float mx[2] = {-INFINITY, -INFINITY};
+  float back[2][2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int at = k0 + 8 * n + 2 * t;
+    const unsigned kb = *reinterpret_cast<const unsigned short*>(scales + at);
+    const unsigned vb = *reinterpret_cast<const unsigned short*>(scales + KEYS + at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int a = (kb >> (8 * i)) & 255, b = (vb >> (8 * i)) & 255;
+      const float up = b == KV8_NAN ? kv8_scale(KV8_NAN) : kv8_scale(a);
+      const float add = b == KV8_NAN ? 0.f : (float)(b - KV8_BIAS);
+      back[n][i] = b == KV8_NAN ? 1.f : __int_as_float((254 - b) << 23);
+      const int key = key0 + 8 * n + 2 * t + i;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float u = c[n][2 * h + i] * up * q.factor[h] + add;
+        if (!clear) {
+          const int pos = h ? pos_b : pos_a;
+          const bool seen = key <= pos && (p.window <= 0 || pos - key < p.window || key < p.keep_first);
+          if (!seen) u = -INFINITY;
+        }
+        c[n][2 * h + i] = u;
+        mx[h] = fmaxf(mx[h], u);
+      }
+    }
+  }
+  float corr[2], base[2], sum[2] = {0.f, 0.f};
+  unsigned a[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+    const float now = fmaxf(s.m[h], mx[h]);
+    corr[h] = s.m[h] == -INFINITY ? 0.f : exp2f(s.m[h] - now);
+    s.m[h] = now;
+    base[h] = now == -INFINITY ? 0.f : now;
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float w0 = exp2f(c[n][2 * h] - base[h]), w1 = exp2f(c[n][2 * h + 1] - base[h]);
+      sum[h] += w0 * back[n][0] + w1 * back[n][1];
+      a[2 * n + h] = pack_half(w0, w1);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) s.l[h] = s.l[h] * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
+  if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) { s.o[n][0] *= corr[0]; s.o[n][1] *= corr[0]; s.o[n][2] *= corr[1]; s.o[n][3] *= corr[1]; }
+  }
+  const unsigned char* vs = stage + MATRIX;
+  value_stretch<0, D >= 128 ? 16 : D >= 64 ? 8 : D >= 32 ? 4 : 2>(vs, k0, a, s.o, lane);
+  if constexpr (D == 256) value_stretch<128, 16>(vs, k0, a, s.o, lane);
+  if constexpr (D > 128 && D < 256 && (D & 64) != 0) value_stretch<128, 8>(vs, k0, a, s.o, lane);
+  if constexpr (D > 64 && (D & 32) != 0) value_stretch<D / 64 * 64, 4>(vs, k0, a, s.o, lane);
+  if constexpr (D > 16 && (D & 16) != 0) value_stretch<D / 32 * 32, 2>(vs, k0, a, s.o, lane);
+}
+
+__device__ __forceinline__ void store_row(const Kv8Attention& p, const Entry& e, int kvh, int row, int d, float v) {
+  const int token = row / p.groups, g = row - token * p.groups;
+  p.out[((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D + d] = __float2bfloat16_rn(v);
+}
+
+// PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of a tile.  Otherwise it takes the (at most
+// 16) rows of an entry, and warp w the keys 16 w .. 16 w + 15 of every tile; the warps' sums join at the end.
+// Key tiles come through a ring of STAGES by asynchronous copies, a page looked up per row.
+// grid: (spans x row tiles, entries, kv heads); a block takes `span` key tiles of its unit.
+template <bool PORTION>
+__global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
+  pdl_trigger();
+  pdl_wait();
+  const int entry = blockIdx.y, kvh = blockIdx.z;
+  const int unit = blockIdx.x / p.spans, piece = blockIdx.x - unit * p.spans;
+  const Entry e(p, entry);
+  const int rows = e.n_new * p.groups;
+  if (rows <= p.row_lo || rows > p.row_hi) return;
+  const int row0 = unit * UNIT;
+  if (row0 >= rows) return;
+  const int rows_end = min(rows, row0 + UNIT);
+  const Walk<KEYS> walk(p, e.start, row0, rows_end);
+  const int pieces = pieces_of(p, walk.count);
+  if (piece >= pieces) return;
+  const int begin = piece * p.span, end = piece == pieces - 1 ? walk.count : begin + p.span;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int* table = p.block_table + (size_t)entry * p.max_pages;
+
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (begin + i < end) load_tile(smem + i * STAGE, p, table, kvh, walk.tile(begin + i) * KEYS, walk.key_lo, walk.key_end, tid);
+    cp_async_commit();
+  }
+  const int wrow0 = PORTION ? row0 + warp * ROWS : row0;
+  Queries q;
+  q.load(p, e, kvh, wrow0, rows_end, lane);
+  // rows past the end take the last row's position; nobody reads them
+  const int last = rows_end - 1;
+  const int pos_a = e.start + min(wrow0 + g, last) / p.groups, pos_b = e.start + min(wrow0 + g + 8, last) / p.groups;
+  const int pos_min = e.start + min(wrow0, last) / p.groups, pos_max = e.start + min(wrow0 + ROWS - 1, last) / p.groups;
+  Sums s;
+  s.clear();
+  for (int i = begin; i < end; ++i) {
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();                 // the tile is here, and the stage filled next is no longer read
+    const int ahead = i + STAGES - 1;
+    if (ahead < end)
+      load_tile(smem + ((ahead - begin) % STAGES) * STAGE, p, table, kvh, walk.tile(ahead) * KEYS, walk.key_lo, walk.key_end, tid);
+    cp_async_commit();
+    const unsigned char* stage = smem + ((i - begin) % STAGES) * STAGE;
+    const int key0 = walk.tile(i) * KEYS;
+    for (int j = PORTION ? 0 : warp; j < (PORTION ? KEYS / 16 : warp + 1); ++j) {
+      const int first = key0 + 16 * j;
+      if (first > pos_max) continue;
+      const bool clear = first + 15 <= pos_min && (p.window <= 0 || pos_max - first < p.window);
+      step16(q, stage, 16 * j, first, p, clear, pos_a, pos_b, s, lane);
+    }
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);
+    s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 2);
+  }
+  float* ws = p.ws + ((((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans + piece) * UNIT * (D + 2);
+  if constexpr (PORTION) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = warp * ROWS + g + 8 * h, row = row0 + r;
+      if (row >= rows_end) continue;
+      const float inv = s.l[h] > 0.f ? 1.f / s.l[h] : (s.l[h] == 0.f ? 0.f : s.l[h]);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int d = value_column(n, c, t);
+          if (pieces == 1) store_row(p, e, kvh, row, d, s.o[n][2 * h + c] * inv);
+          else ws[(size_t)r * D + d] = s.o[n][2 * h + c];
+        }
+      if (pieces > 1 && t == 0) {
+        ws[(size_t)UNIT * D + 2 * r] = s.m[h];
+        ws[(size_t)UNIT * D + 2 * r + 1] = s.l[h];
+      }
+    }
+  } else {
+    __syncthreads();                 // the ring's space takes the warps' sums
+    float* acc = reinterpret_cast<float*>(smem);           // [WARPS][16][D]
+    float* ml = acc + WARPS * ROWS * D;                    // [WARPS][16][2]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = g + 8 * h;
+      if (row0 + r >= rows_end) continue;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc[(warp * ROWS + r) * D + value_column(n, c, t)] = s.o[n][2 * h + c];
+      if (t == 0) {
+        ml[(warp * ROWS + r) * 2] = s.m[h];
+        ml[(warp * ROWS + r) * 2 + 1] = s.l[h];
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < (rows_end - row0) * D; i += THREADS) {
+      const int r = i / D, d = i - r * D;
+      float big = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) big = fmaxf(big, ml[(w * ROWS + r) * 2]);
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float mw = ml[(w * ROWS + r) * 2], lw = ml[(w * ROWS + r) * 2 + 1];
+        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : exp2f(mw - big);
+        num += acc[(w * ROWS + r) * D + d] * f;
+        den += lw * f;
+      }
+      if (pieces == 1) {
+        store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : num / den);
+      } else {
+        ws[(size_t)r * D + d] = num;
+        if (d == 0) { ws[(size_t)UNIT * D + 2 * r] = big; ws[(size_t)UNIT * D + 2 * r + 1] = den; }
+      }
+    }
+  }
+}
+
+// Joins the pieces of a unit's rows, in the order of the keys.  grid: (row tiles, entries, kv heads)
+template <int UNIT, int TILE>
+__global__ void __launch_bounds__(THREADS) attn_kv8_join_kernel(Kv8Attention p) {
+  pdl_trigger();
+  pdl_wait();
+  const int unit = blockIdx.x, entry = blockIdx.y, kvh = blockIdx.z;
+  const Entry e(p, entry);
+  const int rows = e.n_new * p.groups, row0 = unit * UNIT;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 >= rows) return;
+  const int rows_end = min(rows, row0 + UNIT);
+  const Walk<TILE> walk(p, e.start, row0, rows_end);
+  const int pieces = pieces_of(p, walk.count);
+  if (pieces == 1) return;
+  const size_t step = (size_t)UNIT * (D + 2);
+  const float* ws = p.ws + (((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans * step;
+  for (int i = threadIdx.x; i < (rows_end - row0) * D; i += THREADS) {
+    const int r = i / D, d = i - r * D;
+    const float* ml = ws + (size_t)UNIT * D + 2 * r;
+    float big = -INFINITY;
+    for (int s = 0; s < pieces; ++s) big = fmaxf(big, ml[s * step]);
+    float num = 0.f, den = 0.f;
+    for (int s = 0; s < pieces; ++s) {
+      const float m = ml[s * step], l = ml[s * step + 1];
+      const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - big);
+      num += ws[s * step + i] * f;
+      den += l * f;
+    }
+    store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : num / den);
+  }
+}
+
+template <bool PORTION>
+int launch_mma(Kv8Attention p, int entries, int max_new, cudaStream_t stream) {
+  constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
+  const long long max_rows = (long long)max_new * p.groups;
+  p.units = PORTION ? (int)((max_rows + UNIT - 1) / UNIT) : 1;
+  if ((long long)p.units * p.spans > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
+  const cudaError_t err = cudaFuncSetAttribute(attn_kv8_mma_kernel<PORTION>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM);
+  if (err != cudaSuccess) return (int)err;
+  int rc = fe_launch_dependent(attn_kv8_mma_kernel<PORTION>, dim3((unsigned)(p.units * p.spans), (unsigned)entries, (unsigned)p.nkv),
+                               dim3(THREADS), MMA_SMEM, stream, p);
+  if (rc == 0 && p.spans > 1)
+    rc = fe_launch_dependent(attn_kv8_join_kernel<UNIT, KEYS>, dim3((unsigned)p.units, (unsigned)entries, (unsigned)p.nkv), dim3(THREADS), 0,
+                             stream, p);
+  return rc;
+}
+
+}  // namespace
+
+// 32-bit numbers of workspace that `entries` of up to `max_new` tokens need, cut into `spans` pieces.
+FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, int nkv, int groups, int max_new, int spans) {
+  if (spans <= 1) return 0;
+  const long long unit = portion ? ROWS * WARPS : ROWS;
+  const long long units = portion ? ((long long)max_new * groups + unit - 1) / unit : 1;
+  return (long long)entries * nkv * units * spans * unit * (D + 2);
+}
+
+// The entries of a step with at most 16 rows (new tokens x heads per kv head) if single_spans is above zero, the others
+// if portion_spans is; `*_span` key tiles of 64 a block, `*_spans` of them for the longest.
+FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
+                                      const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
+                                      int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new,
+                                      int total_tokens, int window, int keep_first, float scale, int single_span,
+                                      int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
+                                      cudaStream_t stream) {
+  if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
+  if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
+  if (single_spans < 0 || portion_spans < 0 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
+  if ((single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
+  if (entries > 65535 || nkv > 65535 || (long long)max_new * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
+  if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) ||
+      q_stride % 4)
+    return FE_ERR_BAD_ALIGN;
+  Kv8Attention p;
+  p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out;
+  p.k = (const unsigned char*)k; p.v = (const unsigned char*)v; p.ks = (const unsigned char*)ks; p.vs = (const unsigned char*)vs;
+  p.block_table = block_table; p.max_pages = max_pages; p.page_size = page_size; p.num_pages = num_pages;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (page_size == 1 << s) p.page_shift = s;
+  p.nkv = nkv; p.groups = groups; p.cu_tokens = cu_tokens; p.starts = starts; p.total_tokens = total_tokens;
+  p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  p.ws = workspace;
+  if (single_spans > 0) {
+    p.row_lo = 0; p.row_hi = ROWS; p.span = single_span; p.spans = single_spans;
+    const int rc = launch_mma<false>(p, entries, max_new, stream);
+    if (rc) return rc;
+  }
+  if (portion_spans > 0) {
+    p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans;
+    const int rc = launch_mma<true>(p, entries, max_new, stream);
+    if (rc) return rc;
+  }
+  return fe_last_error();
+}

@@ -43,12 +43,16 @@ def find_nvcc() -> str:
 PER_HEAD_DIM = ("attention_mma.cu",)
 
 
+# The same for the 8-bit cache's attention, in libraries of their own.
+PER_HEAD_DIM_KV8 = ("attention_kv8.cu",)
+
+
 # Compiled once per (key size, value size, value-inside-key) of a general attention layer.
 PER_SHAPE = ("attention_general_mma.cu",)
 
 
 def _sources() -> list[Path]:
-    return sorted(p for p in CSRC.glob("*.cu") if p.name not in PER_HEAD_DIM + PER_SHAPE)
+    return sorted(p for p in CSRC.glob("*.cu") if p.name not in PER_HEAD_DIM + PER_HEAD_DIM_KV8 + PER_SHAPE)
 
 
 def _fingerprint(nvcc: str, sources: list, defines: list) -> str:
@@ -135,6 +139,14 @@ def attention_library_path(head_dim: int, verbose: bool = True) -> Path:
         raise CUDAUnavailableError(f"no tensor-core attention for head_dim={head_dim}")
     name = f"libforge_engine_b200_attn_d{head_dim}.so"
     return _build(name, [CSRC / n for n in PER_HEAD_DIM], [f"-DFE_HEAD_DIM={head_dim}"], verbose)
+
+
+def kv8_attention_library_path(head_dim: int, verbose: bool = True) -> Path:
+    """The attention kernels over the 8-bit cache, specialised for one head size."""
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise CUDAUnavailableError(f"no attention over the 8-bit cache for head_dim={head_dim}")
+    name = f"libforge_engine_b200_kv8_d{head_dim}.so"
+    return _build(name, [CSRC / n for n in PER_HEAD_DIM_KV8], [f"-DFE_HEAD_DIM={head_dim}"], verbose)
 
 
 def general_attention_library_path(key_dim: int, value_dim: int, value_in_key: bool, verbose: bool = True) -> Path:

@@ -8,13 +8,14 @@ a CUDA device or without the library these functions raise ``CUDAUnavailableErro
 from __future__ import annotations
 
 import ctypes
+import functools as _functools
 import os as _os
 from ctypes import c_float, c_int, c_ulonglong, c_void_p
 
 import torch
 
 from ..errors import CUDAUnavailableError, ForgeEngineError, UnsupportedShapeError
-from .build import attention_library_path, general_attention_library_path, library_path
+from .build import attention_library_path, general_attention_library_path, kv8_attention_library_path, library_path
 
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -115,6 +116,8 @@ def _declare(handle: ctypes.CDLL) -> None:
         "fe_rglru_scratch": [i, i, i],
         "fe_latent_rows": [p, i, p, i, i, i, p, i, p, p, p, p],
         "fe_rglru_one_launch": [i, i],
+        "fe_kv8_write": [p, ll, p, i, p, ll, p, ll, i, p, p, f, p, i, p, p, p, p, p, p, p, i, i, i, i, i, i, i, p, p],
+        "fe_kv8_read": [p, p, p, p, p, i, i, i, i, i, i, p, p, p, p, i, i, p, p],
         "fe_gemm_tc5_qkv_rope": [p, p, p, p, i, i, i, p, p, f, p, p, p, p, p, p, i, i, i, i, i, i, p, p],
     }
     for name, argtypes in signatures.items():
@@ -1880,3 +1883,228 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor, status: torch.Tensor, w
     rows, vocab = logits.shape
     assert logits.dtype == torch.float32 and out.dtype == torch.int32 and out.numel() >= rows and len(wishes) == 32 * rows
     check(lib().fe_sample_rows(ptr(logits), rows, vocab, wishes, ptr(out), ptr(status), stream()), "sample_rows")
+
+
+# ---------------------------------------------------------------------------
+# the 8-bit cache
+# ---------------------------------------------------------------------------
+
+KV8_CODES, KV8_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
+KV8_SINGLE_ROWS = 16         # rows (new tokens x heads per kv head) of an entry that the kernel of single tokens takes
+KV8_TILE = 64                # keys of a tile
+
+_kv8_handles: dict = {}
+
+
+def kv8_takes(head_dim: int) -> bool:
+    """Whether the 8-bit cache has this head size."""
+    return head_dim % 16 == 0 and 16 <= head_dim <= 256
+
+
+def kv8_lib(head_dim: int):
+    """The attention over the 8-bit cache compiled for ``head_dim`` (built on first use): (call, workspace size)."""
+    got = _kv8_handles.get(head_dim)
+    if got is None:
+        path = kv8_attention_library_path(head_dim)
+        try:
+            handle = ctypes.CDLL(str(path))
+        except OSError as error:
+            raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
+        p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
+        fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, p, p, p]
+        fn.restype = c_int
+        size.argtypes = [i, i, i, i, i, i]
+        size.restype = ll
+        got = _kv8_handles[head_dim] = (fn, size)
+    return got
+
+
+def _kv8_refuse(unless: bool, message: str) -> None:
+    if not unless:
+        raise UnsupportedShapeError(message)
+
+
+def _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status) -> tuple:
+    """(pages, kv heads, page size, head size) after the checks of types and shapes that every call over an 8-bit cache makes."""
+    _kv8_refuse(k_cache.dtype == v_cache.dtype == KV8_CODES and k_scale.dtype == v_scale.dtype == KV8_SCALES,
+                "an 8-bit cache holds float8_e4m3fn codes and float8_e8m0fnu scales")
+    shape = tuple(k_cache.shape)
+    _kv8_refuse(len(shape) == 4 and tuple(v_cache.shape) == shape and tuple(k_scale.shape) == tuple(v_scale.shape) == shape[:3],
+                "an 8-bit cache is [pages, kv heads, page size, head size] codes and [pages, kv heads, page size] scales")
+    _kv8_refuse(kv8_takes(shape[3]), f"head size {shape[3]}: the 8-bit cache takes multiples of 16 up to 256")
+    _kv8_refuse(shape[1] >= 1 and shape[2] >= 1, "an 8-bit cache has kv heads and pages of at least one token")
+    _kv8_refuse(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table is [entries, pages] int32")
+    _kv8_refuse(status.dtype == torch.int32 and status.numel() >= 1, "status is an int32 word")
+    return shape
+
+
+def _kv8_device(first: torch.Tensor, *others, rows=()) -> None:
+    """Everything on one CUDA device, and dense but for ``rows``."""
+    for t in (first, *others):
+        if t is not None and t.numel():
+            _dense(t, "every tensor of a call over the 8-bit cache but k, v and q")
+    for t in (first, *others, *rows):
+        if t is not None and t.device != first.device:
+            raise UnsupportedShapeError(f"tensors on {first.device} and {t.device}: a call works on one device")
+
+
+def _kv8_rows(t: torch.Tensor, n: int, width: int, name: str) -> int:
+    """The distance of the rows of ``t`` [n, width]."""
+    _kv8_refuse(t.dim() == 2 and tuple(t.shape) == (n, width) and (width <= 1 or t.stride(1) == 1),
+                f"{name} must be [{n}, {width}] with neighbouring elements side by side, got {tuple(t.shape)}")
+    return int(t.stride(0)) if n > 1 else width
+
+
+def _kv8_places(positions: torch.Tensor, token_entry: torch.Tensor, n: int) -> None:
+    for t, name in ((positions, "positions"), (token_entry, "token_entry")):
+        _kv8_refuse(t.dtype == torch.int32 and t.numel() == n, f"{name} must hold {n} int32 numbers")
+
+
+def kv8_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.Tensor, token_entry: torch.Tensor,
+              k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+              block_table: torch.Tensor, status: torch.Tensor, *, q: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+              eps: float = 0.0, table: torch.Tensor | None = None) -> None:
+    """Quantise keys and values into their pages of an 8-bit cache.
+
+    ``k``, ``v`` [N, kv heads * D] (bfloat16 or 32-bit, rows any distance apart - column slices of a projection -
+    that is a multiple of four elements; both None: queries only) are token n's vectors, stored at ``positions[n]`` of
+    entry ``token_entry[n]`` of ``block_table``.  Caches: e4m3 codes [pages, kv heads, page_size, D] and e8m0 scales
+    [pages, kv heads, page_size]; a cached number is code * scale, the scale the least power of two (2^-64 to 2^64)
+    for which a vector's largest element is at most 448 of it, rounding to nearest even.  A vector with an
+    infinity or a NaN reads back as NaN.  A place named twice in one call holds either vector, or parts of both.
+
+    ``k_norm`` [D] (32-bit): keys are first normalised per head (root mean square, ``eps``) and multiplied by
+    it.  ``table`` [N, R / 2, 2] (32-bit cosines and sines, R a multiple of 8 up to D): then the first R elements of a
+    head are rotated in halves.  ``q`` [N, heads * D] of the same type goes the same way with ``q_norm`` and is
+    stored in ``q_out`` [N, heads * D] (bfloat16, dense, not overlapping any input).
+
+    A position outside the block table or a missing page sets a bit of ``status`` and writes nothing."""
+    num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
+    _kv8_refuse((k is None) == (v is None) and (q is None) == (q_out is None), "kv8_write: k goes with v, and q with q_out")
+    some = q if k is None else k
+    _kv8_refuse(some is not None, "kv8_write: nothing to write")
+    n = positions.numel()
+    _kv8_places(positions, token_entry, n)
+    k_stride = v_stride = q_stride = heads = 0
+    if k is not None:
+        k_stride, v_stride = _kv8_rows(k, n, nkv * d, "k"), _kv8_rows(v, n, nkv * d, "v")
+    if q is not None:
+        heads = q.shape[-1] // d
+        q_stride = _kv8_rows(q, n, heads * d, "q")
+        _kv8_refuse(q_out.dtype == torch.bfloat16 and q_out.shape == q.shape, "q_out must be bfloat16 of q's shape")
+    _kv8_refuse(all(t is None or t.dtype == some.dtype for t in (k, v, q)), "k, v and q are of one type")
+    some_code = code(some)
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        _kv8_refuse(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (d,)), f"{name} must be 32-bit, [{d}]")
+    _kv8_refuse(table is None or (table.dtype == torch.float32 and table.dim() == 3 and table.shape[0] == n and table.shape[2] == 2),
+                f"table must be 32-bit, [{n}, pairs, 2]")
+    rot = 0 if table is None else 2 * int(table.shape[1])
+    _kv8_refuse(rot <= d and rot % 8 == 0, f"{rot} rotated elements: a multiple of 8 up to the head size {d}")
+    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, q_out, q_norm, k_norm, table,
+                rows=(k, v, q))
+    with torch.cuda.device(k_cache.device):
+        check(lib().fe_kv8_write(ptr(q), q_stride, ptr(q_out), heads, ptr(k), k_stride, ptr(v), v_stride, some_code, ptr(q_norm),
+                                 ptr(k_norm), float(eps), ptr(table) if rot else None, rot, ptr(positions), ptr(token_entry),
+                                 ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table),
+                                 block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, d, n, ptr(status),
+                                 stream()), "kv8_write")
+
+
+def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+             block_table: torch.Tensor, positions: torch.Tensor, token_entry: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor, status: torch.Tensor) -> None:
+    """Read an 8-bit cache back: ``k_out[n]``, ``v_out[n]`` [N, kv heads, D] (bfloat16 or 32-bit; exact in both) are what
+    lies at ``positions[n]`` of entry ``token_entry[n]``.  A position outside the block table or a missing page sets a
+    bit of ``status`` and gives zeros."""
+    num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
+    n = positions.numel()
+    _kv8_places(positions, token_entry, n)
+    _kv8_refuse(k_out.dtype == v_out.dtype and tuple(k_out.shape) == tuple(v_out.shape) == (n, nkv, d),
+                f"k_out and v_out must be [{n}, {nkv}, {d}] of one type")
+    out_code = code(k_out)
+    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, k_out, v_out)
+    with torch.cuda.device(k_cache.device):
+        check(lib().fe_kv8_read(ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table), block_table.shape[0],
+                                block_table.shape[1], page_size, num_pages, nkv, d, ptr(positions), ptr(token_entry), ptr(k_out),
+                                ptr(v_out), out_code, n, ptr(status), stream()), "kv8_read")
+
+
+def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window: int | None = None, keep_first: int = 0) -> tuple:
+    """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries: (key tiles a
+    block takes of an entry with at most 16 rows, such blocks of the longest one, and both for the other entries);
+    a count of 0: there is no such entry.  Layers of one geometry share it."""
+    return _kv8_plan(tuple((int(start), int(count)) for start, count in entries), int(num_q_heads) // int(num_kv_heads),
+                     int(num_kv_heads), int(head_dim), int(window or 0), int(keep_first or 0))
+
+
+def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, tile: int) -> int:
+    """Key tiles that the queries at positions start + first .. start + last see."""
+    low = max(0, start + first - window + 1) // tile if window else 0
+    kept = min(-(-keep_first // tile), low) if window else 0
+    return kept + -(-(start + last + 1) // tile) - low
+
+
+@_functools.lru_cache(maxsize=4096)
+def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int, keep_first: int) -> tuple:
+    single, portion = [], []
+    for start, count in entries:
+        rows = count * groups
+        if rows <= 0:
+            continue
+        if rows <= KV8_SINGLE_ROWS:
+            single.append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
+        else:
+            for row in range(0, rows, 64):
+                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + 64) - 1) // groups, window, keep_first, KV8_TILE))
+    plan = []
+    for tiles, slots in ((single, 444), (portion, 296)):
+        span, spans = _kv8_cut(tuple(sorted(tiles)), nkv, slots) if tiles else (1, 0)
+        plan += [span, spans]
+    return tuple(plan)
+
+
+def _kv8_cut(tiles: tuple, nkv: int, slots: int) -> tuple:
+    longest = tiles[-1]
+    span = 1
+    while span < longest and nkv * sum(-(-t // span) for t in tiles) > slots:
+        span += max(1, span // 4)
+    spans = -(-longest // span)
+    return (longest, 1) if spans <= 1 else (span, 1 << (spans - 1).bit_length())
+
+
+def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_table: torch.Tensor, cu_tokens: torch.Tensor, starts: torch.Tensor, n_entries: int, max_new: int,
+                  num_q_heads: int, window: int | None, keep_first: int, scale: float, out: torch.Tensor, status: torch.Tensor,
+                  plan: tuple) -> None:
+    """Causal grouped-query attention over an 8-bit cache (``kv8_write``), which holds the new tokens already.
+
+    ``q`` [N, heads * D] (bfloat16; rows any multiple of four elements apart) are the queries of ``n_entries`` entries:
+    entry e's are rows ``cu_tokens[e]`` .. ``cu_tokens[e + 1]``, at positions ``starts[e]`` on (``cu_tokens``, ``starts``
+    int32 on the device; at most ``max_new`` rows an entry).  A query sees every key up to its own, or with ``window``
+    the last ``window`` of them and the first ``keep_first`` of the sequence.  ``out`` [N, heads * D] (bfloat16, dense); rows
+    of no entry are left as they are.  ``plan``: ``kv8_plan`` of these entries.  32-bit scores, softmax and sums."""
+    num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
+    n_entries, max_new, window, keep_first = int(n_entries), int(max_new), int(window or 0), int(keep_first or 0)
+    n = q.shape[0]
+    _kv8_refuse(num_q_heads >= 1 and num_q_heads % nkv == 0, f"{num_q_heads} heads over {nkv} kv heads")
+    q_stride = _kv8_rows(q, n, num_q_heads * d, "q")
+    _kv8_refuse(q.dtype == out.dtype == torch.bfloat16 and out.shape == q.shape, "q and out are bfloat16 of one shape")
+    _kv8_refuse(n_entries >= 0 and max_new >= 0 and window >= 0 and keep_first >= 0, "attention_kv8: no negative sizes")
+    _kv8_refuse(cu_tokens.dtype == starts.dtype == torch.int32 and cu_tokens.numel() > n_entries and starts.numel() >= n_entries,
+                "cu_tokens holds entries + 1 int32 numbers, starts one an entry")
+    _kv8_refuse(block_table.shape[0] >= n_entries, "attention_kv8: a block table row per entry")
+    _kv8_refuse(scale > 0, "attention_kv8: the scale is positive")
+    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out, rows=(q,))
+    single_span, single_spans, portion_span, portion_spans = plan
+    groups = num_q_heads // nkv
+    fn, size = kv8_lib(d)
+    with torch.cuda.device(q.device):
+        # the pieces of a cut entry meet in a buffer of the call's own: calls on other streams, and captured ones, have theirs
+        numbers = max(size(0, n_entries, nkv, groups, max_new, single_spans), size(1, n_entries, nkv, groups, max_new, portion_spans))
+        workspace = torch.empty(numbers, dtype=torch.float32, device=q.device) if numbers else None
+        check(fn(ptr(q), q_stride, ptr(out), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table),
+                 block_table.shape[1], page_size, num_pages, nkv, groups, ptr(cu_tokens), ptr(starts), n_entries, max_new, n, window,
+                 keep_first, float(scale), single_span, single_spans, portion_span, portion_spans, ptr(workspace), ptr(status),
+                 stream()), "attention_kv8")
