@@ -1,5 +1,6 @@
 // Causal grouped-query attention over the 8-bit cache (layout: kv8.cuh), compiled for one head size:
-// -DFE_HEAD_DIM=<multiple of 16, 16..256>.
+// -DFE_HEAD_DIM=<multiple of 16, 16..256>.  Single tokens of every head size and portions of head sizes other than 64
+// and 128, which attention_kv8_portion.cu takes.
 //
 // A query at position i of a sequence sees the keys j <= i, or with a window those of the last `window`
 // positions and the first `keep_first`.  With cached key code c_j, value code d_j and their scales 2^a_j, 2^b_j:
@@ -18,19 +19,16 @@
 // src/forge_engine/qwen3.py:187-206 and the decode kernel of src/forge_engine/kernels/cuda_paged.py:276-347.
 #include <cuda_fp16.h>
 
-#include "kv8.cuh"
+#include "attention_kv8.cuh"
 
-#ifndef FE_HEAD_DIM
-#error "compile with -DFE_HEAD_DIM=<head size>"
-#endif
 #define CAT_(a, b) a##b
 #define CAT(a, b) CAT_(a, b)
 #define SYM(name) CAT(name, FE_HEAD_DIM)
 
+using namespace kv8;
+
 namespace {
 
-constexpr int D = FE_HEAD_DIM;
-static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 up to 256");
 constexpr int CHUNKS = D / 16;          // 16-byte pieces of a cached vector
 constexpr int KEYS = 64;                // keys of a tile
 constexpr int ROWS = 16;                // rows a warp takes: the m of one mma
@@ -41,24 +39,6 @@ constexpr int STAGE = 2 * MATRIX + 2 * KEYS;
 constexpr size_t MMA_SMEM_RING = (size_t)STAGES * STAGE;
 constexpr size_t MMA_SMEM_JOIN = (size_t)WARPS * ROWS * (D + 2) * sizeof(float);
 constexpr size_t MMA_SMEM = MMA_SMEM_RING > MMA_SMEM_JOIN ? MMA_SMEM_RING : MMA_SMEM_JOIN;
-
-struct Kv8Attention {
-  const bf16* q;
-  long long q_stride;
-  bf16* out;               // [tokens, nkv * groups * D]
-  const unsigned char *k, *v, *ks, *vs;
-  const int* block_table;
-  int max_pages, page_size, page_shift, num_pages, nkv, groups;
-  const int* cu_tokens;    // [entries + 1]
-  const int* starts;       // [entries]
-  int total_tokens, window, keep_first;
-  float scale_log2;
-  int* status;
-  int row_lo, row_hi;      // entries with row_lo < rows <= row_hi
-  int span, spans;         // a block takes `span` key tiles of a unit; the grid holds `spans` of them
-  int units;               // row tiles of the longest entry
-  float* ws;               // [entries, nkv, units, spans, rows of a unit, D + 2]: sums, then M and l
-};
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
@@ -79,51 +59,6 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 
-// The key tiles (of TILE keys) that the rows [row0, row0 + n) of an entry see: first the tiles that hold kept
-// first tokens and lie before the window, then the window's.
-template <int TILE>
-struct Walk {
-  int pos_first, pos_last, key_lo, key_end, kept, first, count;
-  __device__ __forceinline__ Walk(const Kv8Attention& p, int start, int row0, int rows_end) {
-    pos_first = start + row0 / p.groups;
-    pos_last = start + (rows_end - 1) / p.groups;
-    key_lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
-    key_end = pos_last + 1;
-    first = key_lo / TILE;
-    kept = p.window > 0 ? min((p.keep_first + TILE - 1) / TILE, first) : 0;
-    count = kept + (key_end + TILE - 1) / TILE - first;
-  }
-  __device__ __forceinline__ int tile(int i) const { return i < kept ? i : first + i - kept; }
-};
-
-// Pieces of a unit of `count` key tiles; where the grid holds fewer than its spans give, the last takes the rest.
-__device__ __forceinline__ int pieces_of(const Kv8Attention& p, int count) { return min(p.spans, (count + p.span - 1) / p.span); }
-
-// Tokens of an entry, held to the tensors the call brought.
-struct Entry {
-  int tok0, n_new, start;
-  __device__ __forceinline__ Entry(const Kv8Attention& p, int entry) {
-    tok0 = p.cu_tokens[entry];
-    n_new = p.cu_tokens[entry + 1] - tok0;
-    start = p.starts[entry];
-    if (tok0 < 0 || n_new < 0 || tok0 > p.total_tokens - n_new || start < 0 || start > 0x7fff0000 - n_new) {
-      if (threadIdx.x == 0) atomicOr(p.status, FE_STATUS_BAD_POSITION);
-      n_new = 0;
-    }
-  }
-};
-
-// Row (page, head, slot) of a key, or -1 where its page is missing (flagged if some row must see it).
-__device__ __forceinline__ long long key_row(const Kv8Attention& p, const int* table, int kvh, int key, bool needed) {
-  const int logical = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-  const int page = logical < p.max_pages ? table[logical] : -1;
-  if (page < 0 || page >= p.num_pages) {
-    if (needed) atomicOr(p.status, FE_STATUS_BAD_PAGE);
-    return -1;
-  }
-  return ((long long)page * p.nkv + kvh) * p.page_size + (key - logical * p.page_size);
-}
-
 // Where 16-byte piece c of row r lies.  Keys are read 8 rows x 4 pieces at a time (rows two by two in a phase
 // of a shared-memory read), values the rows 2t, 2t + 1, 2t + 8, 2t + 9 x pieces of 8 lanes: each matrix has the
 // exchange of pieces that keeps its reads apart.  Head sizes without a whole power of two of pieces take none.
@@ -132,35 +67,51 @@ __device__ __forceinline__ int value_piece(int r, int c) {
   return D % 128 == 0 ? c ^ (((r >> 1) & 3) << 1) : D % 64 == 0 ? c ^ ((r >> 1) & 3) : c;
 }
 
-// Stage the keys [key0, key0 + 64) of one kv head, their values and both scales.  What lies at or past key_end
-// is zero.
-__device__ __forceinline__ void load_tile(unsigned char* stage, const Kv8Attention& p, const int* table, int kvh, int key0,
-                                          int key_lo, int key_end, int tid) {
-  unsigned char* kd = stage;
-  unsigned char* vd = stage + MATRIX;
-  unsigned char* sd = stage + 2 * MATRIX;
+// Stages tiles of 64 keys of one kv head, their values and both scales.  What lies at or past key_end is zero.  A
+// thread copies 16-byte pieces of up to COPIES rows; the rows' pages are looked up a tile ahead.
+struct Staging {
+  static constexpr int COPIES = (KEYS * CHUNKS + THREADS - 1) / THREADS;
+  int pages[COPIES], scale_page;
+
+  static __device__ __forceinline__ int scale_row(const Kv8Attention& p, int tid) {
+    return p.page_size % 4 == 0 ? (tid % (KEYS / 4)) * 4 : tid % KEYS;
+  }
+
+  __device__ __forceinline__ void look_up(const Kv8Attention& p, const int* table, int key0, int key_end, int tid) {
 #pragma unroll
-  for (int u = tid; u < KEYS * CHUNKS; u += THREADS) {
-    const int row = u / CHUNKS, c = u - row * CHUNKS, key = key0 + row;
-    long long at = key < key_end ? key_row(p, table, kvh, key, c == 0 && (key >= key_lo || key < p.keep_first)) : -1;
-    const bool valid = at >= 0;
-    if (!valid) at = 0;
-    cp_async16(kd + row * D + key_piece(row, c) * 16, p.k + at * D + c * 16, valid);
-    cp_async16(vd + row * D + value_piece(row, c) * 16, p.v + at * D + c * 16, valid);
-  }
-  if (p.page_size % 4 == 0) {          // four neighbouring scales lie in one word
-    if (tid < 2 * (KEYS / 4)) {
-      const int row = (tid % (KEYS / 4)) * 4, m = tid / (KEYS / 4), key = key0 + row;
-      long long at = key < key_end ? key_row(p, table, kvh, key, false) : -1;
-      const bool valid = at >= 0;
-      cp_async4(sd + m * KEYS + row, (m ? p.vs : p.ks) + (valid ? at : 0), valid);
+    for (int j = 0; j < COPIES; ++j) {
+      const int row = (tid + j * THREADS) / CHUNKS;
+      pages[j] = row < KEYS ? key_page(p, table, key0 + row, key_end) : -1;
     }
-  } else {
-    const int row = tid % KEYS, m = tid / KEYS, key = key0 + row;
-    const long long at = key < key_end ? key_row(p, table, kvh, key, false) : -1;
-    sd[m * KEYS + row] = at >= 0 ? (m ? p.vs : p.ks)[at] : 0;
+    scale_page = key_page(p, table, key0 + scale_row(p, tid), key_end);
   }
-}
+
+  __device__ __forceinline__ void copy(unsigned char* stage, const Kv8Attention& p, int kvh, int key0, int key_lo, int key_end, int tid) const {
+    unsigned char* kd = stage;
+    unsigned char* vd = stage + MATRIX;
+    unsigned char* sd = stage + 2 * MATRIX;
+#pragma unroll
+    for (int j = 0; j < COPIES; ++j) {
+      const int u = tid + j * THREADS, row = u / CHUNKS, c = u - row * CHUNKS;
+      if (KEYS * CHUNKS % THREADS != 0 && row >= KEYS) break;
+      long long at;
+      const bool there = key_row(p, pages[j], kvh, key0 + row, &at);
+      if (!there && c == 0) tell_missing(p, key0 + row, key_lo, key_end);
+      cp_async16(kd + row * D + key_piece(row, c) * 16, p.k + at * D + c * 16, there);
+      cp_async16(vd + row * D + value_piece(row, c) * 16, p.v + at * D + c * 16, there);
+    }
+    const int row = scale_row(p, tid);
+    long long at;
+    const bool there = key_row(p, scale_page, kvh, key0 + row, &at);
+    if (p.page_size % 4 == 0) {          // four neighbouring scales lie in one word
+      const int m = tid / (KEYS / 4);
+      if (m < 2) cp_async4(sd + m * KEYS + row, (m ? p.vs : p.ks) + at, there);
+    } else {
+      const int m = tid / KEYS;
+      sd[m * KEYS + row] = there ? (m ? p.vs : p.ks)[at] : 0;
+    }
+  }
+};
 
 // The queries of a warp's 16 rows as the A operand.  The order of the contraction is free as long as both
 // operands keep it: in every stretch of 64 elements lane t of a quad holds elements 16 t .. 16 t + 15, which it
@@ -360,11 +311,6 @@ __device__ __forceinline__ void step16(const Queries& q, const unsigned char* st
   if constexpr (D > 16 && (D & 16) != 0) value_stretch<D / 32 * 32, 2>(vs, k0, a, s.o, lane);
 }
 
-__device__ __forceinline__ void store_row(const Kv8Attention& p, const Entry& e, int kvh, int row, int d, float v) {
-  const int token = row / p.groups, g = row - token * p.groups;
-  p.out[((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D + d] = __float2bfloat16_rn(v);
-}
-
 // PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of a tile.  Otherwise it takes the (at most
 // 16) rows of an entry, and warp w the keys 16 w .. 16 w + 15 of every tile; the warps' sums join at the end.
 // Key tiles come through a ring of STAGES by asynchronous copies, a page looked up per row.
@@ -390,11 +336,17 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int* table = p.block_table + (size_t)entry * p.max_pages;
 
+  auto key0_of = [&](int i) -> int { return walk.tile(i) * KEYS; };
+  Staging staging[STAGES - 1];           // all lookups of the first tiles at once
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) staging[i].look_up(p, table, key0_of(min(begin + i, end - 1)), walk.key_end, tid);
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
-    if (begin + i < end) load_tile(smem + i * STAGE, p, table, kvh, walk.tile(begin + i) * KEYS, walk.key_lo, walk.key_end, tid);
+    if (begin + i < end) staging[i].copy(smem + i * STAGE, p, kvh, key0_of(begin + i), walk.key_lo, walk.key_end, tid);
     cp_async_commit();
   }
+  Staging& next = staging[0];
+  next.look_up(p, table, key0_of(min(begin + STAGES - 1, end - 1)), walk.key_end, tid);
   const int wrow0 = PORTION ? row0 + warp * ROWS : row0;
   Queries q;
   q.load(p, e, kvh, wrow0, rows_end, lane);
@@ -408,9 +360,9 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
     cp_async_wait<STAGES - 2>();
     __syncthreads();                 // the tile is here, and the stage filled next is no longer read
     const int ahead = i + STAGES - 1;
-    if (ahead < end)
-      load_tile(smem + ((ahead - begin) % STAGES) * STAGE, p, table, kvh, walk.tile(ahead) * KEYS, walk.key_lo, walk.key_end, tid);
+    if (ahead < end) next.copy(smem + ((ahead - begin) % STAGES) * STAGE, p, kvh, key0_of(ahead), walk.key_lo, walk.key_end, tid);
     cp_async_commit();
+    if (ahead + 1 < end) next.look_up(p, table, key0_of(ahead + 1), walk.key_end, tid);
     const unsigned char* stage = smem + ((i - begin) % STAGES) * STAGE;
     const int key0 = walk.tile(i) * KEYS;
     for (int j = PORTION ? 0 : warp; j < (PORTION ? KEYS / 16 : warp + 1); ++j) {
@@ -439,7 +391,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
         for (int c = 0; c < 2; ++c) {
           const int d = value_column(n, c, t);
           if (pieces == 1) store_row(p, e, kvh, row, d, s.o[n][2 * h + c] * inv);
-          else ws[(size_t)r * D + d] = s.o[n][2 * h + c];
+          else ws[piece_element<UNIT>(r, d)] = s.o[n][2 * h + c];
         }
       if (pieces > 1 && t == 0) {
         ws[(size_t)UNIT * D + 2 * r] = s.m[h];
@@ -473,48 +425,17 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float mw = ml[(w * ROWS + r) * 2], lw = ml[(w * ROWS + r) * 2 + 1];
-        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : exp2f(mw - big);
+        const float f = piece_share(mw, lw, big);
         num += acc[(w * ROWS + r) * D + d] * f;
         den += lw * f;
       }
       if (pieces == 1) {
         store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : num / den);
       } else {
-        ws[(size_t)r * D + d] = num;
+        ws[piece_element<UNIT>(r, d)] = num;
         if (d == 0) { ws[(size_t)UNIT * D + 2 * r] = big; ws[(size_t)UNIT * D + 2 * r + 1] = den; }
       }
     }
-  }
-}
-
-// Joins the pieces of a unit's rows, in the order of the keys.  grid: (row tiles, entries, kv heads)
-template <int UNIT, int TILE>
-__global__ void __launch_bounds__(THREADS) attn_kv8_join_kernel(Kv8Attention p) {
-  pdl_trigger();
-  pdl_wait();
-  const int unit = blockIdx.x, entry = blockIdx.y, kvh = blockIdx.z;
-  const Entry e(p, entry);
-  const int rows = e.n_new * p.groups, row0 = unit * UNIT;
-  if (rows <= p.row_lo || rows > p.row_hi || row0 >= rows) return;
-  const int rows_end = min(rows, row0 + UNIT);
-  const Walk<TILE> walk(p, e.start, row0, rows_end);
-  const int pieces = pieces_of(p, walk.count);
-  if (pieces == 1) return;
-  const size_t step = (size_t)UNIT * (D + 2);
-  const float* ws = p.ws + (((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans * step;
-  for (int i = threadIdx.x; i < (rows_end - row0) * D; i += THREADS) {
-    const int r = i / D, d = i - r * D;
-    const float* ml = ws + (size_t)UNIT * D + 2 * r;
-    float big = -INFINITY;
-    for (int s = 0; s < pieces; ++s) big = fmaxf(big, ml[s * step]);
-    float num = 0.f, den = 0.f;
-    for (int s = 0; s < pieces; ++s) {
-      const float m = ml[s * step], l = ml[s * step + 1];
-      const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - big);
-      num += ws[s * step + i] * f;
-      den += l * f;
-    }
-    store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : num / den);
   }
 }
 
@@ -529,8 +450,8 @@ int launch_mma(Kv8Attention p, int entries, int max_new, cudaStream_t stream) {
   int rc = fe_launch_dependent(attn_kv8_mma_kernel<PORTION>, dim3((unsigned)(p.units * p.spans), (unsigned)entries, (unsigned)p.nkv),
                                dim3(THREADS), MMA_SMEM, stream, p);
   if (rc == 0 && p.spans > 1)
-    rc = fe_launch_dependent(attn_kv8_join_kernel<UNIT, KEYS>, dim3((unsigned)p.units, (unsigned)entries, (unsigned)p.nkv), dim3(THREADS), 0,
-                             stream, p);
+    rc = fe_launch_dependent(attn_kv8_join_kernel<UNIT, KEYS>, dim3((unsigned)(p.units * (UNIT / JOIN_WARPS)), (unsigned)entries, (unsigned)p.nkv),
+                             dim3(32 * JOIN_WARPS), 0, stream, p);
   return rc;
 }
 
@@ -539,13 +460,18 @@ int launch_mma(Kv8Attention p, int entries, int max_new, cudaStream_t stream) {
 // 32-bit numbers of workspace that `entries` of up to `max_new` tokens need, cut into `spans` pieces.
 FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, int nkv, int groups, int max_new, int spans) {
   if (spans <= 1) return 0;
+#if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
+  const long long unit = portion ? PORTION_UNIT : ROWS;
+#else
   const long long unit = portion ? ROWS * WARPS : ROWS;
+#endif
   const long long units = portion ? ((long long)max_new * groups + unit - 1) / unit : 1;
   return (long long)entries * nkv * units * spans * unit * (D + 2);
 }
 
 // The entries of a step with at most 16 rows (new tokens x heads per kv head) if single_spans is above zero, the others
-// if portion_spans is; `*_span` key tiles of 64 a block, `*_spans` of them for the longest.
+// if portion_spans is; `*_span` key tiles a block (of 64 keys, of 128 in the tcgen05 kernel of portions), `*_spans` of
+// them for the longest.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
                                       int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new,
@@ -577,7 +503,11 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   }
   if (portion_spans > 0) {
     p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans;
+#if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
+    const int rc = launch_portion(p, entries, max_new, stream);
+#else
     const int rc = launch_mma<true>(p, entries, max_new, stream);
+#endif
     if (rc) return rc;
   }
   return fe_last_error();

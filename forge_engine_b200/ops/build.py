@@ -44,7 +44,7 @@ PER_HEAD_DIM = ("attention_mma.cu",)
 
 
 # The same for the 8-bit cache's attention, in libraries of their own.
-PER_HEAD_DIM_KV8 = ("attention_kv8.cu",)
+PER_HEAD_DIM_KV8 = ("attention_kv8.cu", "attention_kv8_portion.cu")
 
 
 # Compiled once per (key size, value size, value-inside-key) of a general attention layer.

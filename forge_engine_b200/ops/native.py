@@ -1892,6 +1892,7 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor, status: torch.Tensor, w
 KV8_CODES, KV8_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_SINGLE_ROWS = 16         # rows (new tokens x heads per kv head) of an entry that the kernel of single tokens takes
 KV8_TILE = 64                # keys of a tile
+KV8_TC5_DIMS = (64, 128)     # head sizes whose portions the tcgen05 kernel takes
 
 _kv8_handles: dict = {}
 
@@ -2048,30 +2049,38 @@ def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, 
 
 @_functools.lru_cache(maxsize=4096)
 def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int, keep_first: int) -> tuple:
+    rows_of, tile, slots = (256, 128, 148) if head_dim in KV8_TC5_DIMS else (64, KV8_TILE, 296)
     single, portion = [], []
     for start, count in entries:
         rows = count * groups
-        if rows <= 0:
-            continue
-        if rows <= KV8_SINGLE_ROWS:
+        if 0 < rows <= KV8_SINGLE_ROWS:
             single.append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
-        else:
-            for row in range(0, rows, 64):
-                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + 64) - 1) // groups, window, keep_first, KV8_TILE))
-    plan = []
-    for tiles, slots in ((single, 444), (portion, 296)):
-        span, spans = _kv8_cut(tuple(sorted(tiles)), nkv, slots) if tiles else (1, 0)
-        plan += [span, spans]
-    return tuple(plan)
+        elif rows:
+            for row in range(0, rows, rows_of):
+                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, tile))
+    return (*_kv8_cut(single, nkv, 444, 2.0, 4.0), *_kv8_cut(portion, nkv, slots, 3.0, 4.0))
 
 
-def _kv8_cut(tiles: tuple, nkv: int, slots: int) -> tuple:
-    longest = tiles[-1]
+def _kv8_cut(tiles: list, nkv: int, slots: int, start: float, join: float) -> tuple:
+    """(key tiles a block takes, blocks of the longest unit, rounded up to a power of two) for units of so many tiles per
+    kv head, so that the longest block and all blocks over the ``slots`` that run at once end soonest.  A block costs
+    ``start`` tiles beside its own, joining pieces ``join`` once."""
+    if not tiles:
+        return 1, 0
+    longest = max(tiles)
+    best = None
     span = 1
-    while span < longest and nkv * sum(-(-t // span) for t in tiles) > slots:
-        span += max(1, span // 4)
-    spans = -(-longest // span)
-    return (longest, 1) if spans <= 1 else (span, 1 << (spans - 1).bit_length())
+    while True:
+        span = min(span, longest)
+        pieces = sum(-(-t // span) for t in tiles) * nkv
+        cost = max(span + start, (sum(tiles) * nkv + start * pieces) / slots) + (join if span < longest else 0.0)
+        if best is None or cost < best[0]:
+            best = (cost, span)
+        if span == longest:
+            break
+        span += max(1, span // 8)
+    span = best[1]
+    return span, 1 << (-(-longest // span) - 1).bit_length()
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,

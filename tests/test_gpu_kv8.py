@@ -4,7 +4,7 @@ Bounds.  A stored number is off by at most half a step of e4m3: 2^-4 of it, or 2
 2^-6.  Attention: weights are rounded to half precision (2^-11 of each, and below 2^-14 of the largest
 contribution by what ``plain_kv8.attention`` derives as floor), scores and sums are 32-bit (a score of some tens
 is off by about 2^-18), and the output is rounded to bfloat16 (2^-8): with A = (2^-11 + 2^-12) * sum of
-weight * |value| + floor an output is within A + 2^-8 (|out| + A).  (The floor belongs to it: where one key has
+weight * |value| + floor an output (portions with heads of 64 and 128: weights rounded to bfloat16, A = (2^-8 + 2^-12) * sum) is within A + 2^-8 (|out| + A).  (The floor belongs to it: where one key has
 nearly all the weight and an element of its value is zero, that element consists of what is rounded there.
 Below bfloat16's normal numbers half a step is 2^-134, whatever the value.)"""
 
@@ -205,7 +205,8 @@ def check_attention(cache, requests, q, out, window, keep, scale, large_scores=F
         want, size, floor = plain.attention(q[at : at + n].view(n, -1, dim), k[: start + n], v[: start + n], start, scale, window, keep)
         got = out[at : at + n].double().view(n, -1, dim)
         at += n
-        a = (2.0 ** -11 + 2.0 ** -12) * size + floor
+        brain = dim in (64, 128) and n * (want.shape[1] // k.shape[1]) > 16
+        a = (2.0 ** -8 + 2.0 ** -12) * size if brain else (2.0 ** -11 + 2.0 ** -12) * size + floor
         if large_scores:
             spread = torch.einsum("nkgd,lkd->nkgl", q[at - n : at].double().view(n, k.shape[1], -1, dim).abs(), k[: start + n].abs())
             spread = spread.amax(-1).flatten(1)[..., None] * scale / math.log(2)

@@ -121,9 +121,7 @@ def test_plans_cover_every_key(entries, window, keep) -> None:
         rows = [n * groups for _, n in entries]
         assert (single_spans > 0) == any(0 < r <= 16 for r in rows) and (portion_spans > 0) == any(r > 16 for r in rows)
         for (start, n), r in zip(entries, rows):
-            if r == 0:
-                continue
-            span, spans = (single_span, single_spans) if r <= 16 else (portion_span, portion_spans)
-            assert span >= 1 and spans >= 1 and (spans & (spans - 1)) == 0
-            keys = start + n if not window else min(start + n, window + n + keep + 512)
-            assert span * spans * native.KV8_TILE >= min(keys, start + n) or window
+            if r and not window:
+                span, spans = (single_span, single_spans) if r <= 16 else (portion_span, portion_spans)
+                tile = 128 if r > 16 and dim in native.KV8_TC5_DIMS else native.KV8_TILE
+                assert span >= 1 and spans >= 1 and (spans & (spans - 1)) == 0 and span * spans * tile >= start + n
