@@ -7,10 +7,14 @@
 //           rounded, and what the rounding left.  Together they hold bfloat16's 8 bits down to 2^-11 of the row's
 //           largest element, and what is smaller to within 2^-18 of it, so the scores are products of 8-bit numbers
 //           with the cached codes as they lie in their pages: keys are only copied.  Then softmax, a thread a row: scores from tensor memory times the keys' scales,
-//           mask, running maximum (moved only when it grows by more than 2^8), weights back over the scores as bfloat16
-//   warps 8-14   copy the keys of a tile, and bring its values: 16-byte pieces of codes into registers a tile ahead,
+//           mask, running maximum (moved only when it grows by more than 2^8), weights back over the scores as bfloat16.
+//           A tile is taken in halves of 64 keys: while a half is in the softmax the tensor core works on the other
+//   warps 8-15   copy the keys of a tile, and bring its values: 16-byte pieces of codes into registers a tile ahead,
 //           code * 2^b as bfloat16 (exact) into the swizzled tile in shared memory
-//   warp 15   S_x = Q_x K^T into tensor memory (both parts of the queries), O_x += P_x V with P from tensor memory
+//   warps 16, 17   issue the products of tile 0 and tile 1: O_x += P_x V with P from tensor memory, then in the weights'
+//           place the scores S_x = Q_x K^T (both parts of the queries) of the next tile's half.  A thread that issues
+//           products waits for the tensor core most of the time: one for both tiles left the tensor core idle while it
+//           waited for weights (5,700 cycles a tile), and a softmax thread that did it held up its row's warp (10,000)
 //
 // Values are not left as 8-bit numbers, because then the weights would have to be: a weight as two e4m3 numbers costs
 // a softmax thread more than the 256 rows' share of converting a value.  Measured with keys converted like the
@@ -28,9 +32,9 @@ using namespace kv8;
 namespace {
 
 constexpr int TILE_ROWS = 128, KEYS = PORTION_TILE;
-constexpr int SOFTMAX_WARPS = 8, STAGING_WARPS = 7;
-constexpr int MMA_WARP = SOFTMAX_WARPS + STAGING_WARPS;
-constexpr int THREADS = 32 * (MMA_WARP + 1);
+constexpr int SOFTMAX_WARPS = 8, STAGING_WARPS = 6;
+constexpr int MMA_WARP = SOFTMAX_WARPS + STAGING_WARPS;      // and the next one; the first also takes and frees tensor memory
+constexpr int THREADS = 32 * (MMA_WARP + 2);
 constexpr int K_STAGES = 3, V_STAGES = 3, CK_STAGES = 4;
 constexpr int HALF = KEYS / 2;                    // keys of a softmax step: a tile is taken in two
 constexpr int TMEM_COLS = 512, COL_S = 0, COL_O = 256;     // + 128 x, scores + 64 for the second half
@@ -178,14 +182,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   float* k_factor = reinterpret_cast<float*>(v_tiles + V_STAGES * V_BYTES);      // [stages][128 keys] scales
   uint64_t* k_full = reinterpret_cast<uint64_t*>(k_factor + CK_STAGES * KEYS);   // [stages]
   uint64_t* v_full = k_full + K_STAGES;          // [stages]
-  // freed[n & 3], event n: the tensor core is done with the scores of step n and the value products of step n - 1
+  // freed[n & 3], event n: for every query tile the tensor core is done with the scores of step n and the value
+  // products of step n - 1
   uint64_t* freed = v_full + V_STAGES;           // [4]
   uint64_t* s_full = freed + 4;                  // [2 query tiles][2 halves] scores are there
   uint64_t* p_full = s_full + 4;                 // [2][2] weights are there
-  uint64_t* pv_done = p_full + 4;                // [2][2] and have been multiplied
-  uint64_t* q_full = pv_done + 4;                // [2]
-  uint64_t* o_full = q_full + 2;
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_full + 1);
+  uint64_t* q_full = p_full + 4;                 // [2]
+  uint64_t* o_full = q_full + 2;                 // [2]
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   pdl_trigger();
@@ -215,10 +219,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   if (threadIdx.x == 0) {
     for (int s = 0; s < K_STAGES; ++s) tc5::mbar_init(k_full + s, STAGING_WARPS);
     for (int s = 0; s < V_STAGES; ++s) tc5::mbar_init(v_full + s, STAGING_WARPS);
-    for (int s = 0; s < 4; ++s) tc5::mbar_init(freed + s, 1);
-    for (int x = 0; x < 4; ++x) { tc5::mbar_init(s_full + x, 1); tc5::mbar_init(p_full + x, 4); tc5::mbar_init(pv_done + x, 1); }
-    for (int x = 0; x < 2; ++x) tc5::mbar_init(q_full + x, 4);
-    tc5::mbar_init(o_full, 1);
+    for (int s = 0; s < 4; ++s) tc5::mbar_init(freed + s, t1.valid ? 2 : 1);
+    for (int x = 0; x < 4; ++x) { tc5::mbar_init(s_full + x, 1); tc5::mbar_init(p_full + x, 4); }
+    for (int x = 0; x < 2; ++x) { tc5::mbar_init(q_full + x, 4); tc5::mbar_init(o_full + x, 1); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   if (warp >= SOFTMAX_WARPS && warp < MMA_WARP) {
     // ---- staging ----
     const int* table = p.block_table + (size_t)entry * p.max_pages;
-    // Piece j of this lane is 16 bytes of one of the warp's rows, unit w + 7 j; the lanes of a unit lie so that eight
+    // Piece j of this lane is 16 bytes of one of the warp's rows, unit w + 8 j; the lanes of a unit lie so that eight
     // neighbours store their 32 bytes of bfloat16 without meeting in a bank.  A lane looks after one of the warp's
     // rows - its page, its place and its scales - and the others ask it.
     constexpr int UNIT_ROWS = 32 / CHUNKS;
@@ -243,9 +246,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
     const int w = warp - SOFTMAX_WARPS;
     const int c = CHUNKS == 8 ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane & 3;
     const int sub = CHUNKS == 8 ? ((lane >> 2) & 1) | (lane >> 4) << 1 : lane >> 2;        // row inside the unit
-    const int my_row = lane < PIECES * UNIT_ROWS ? (w + STAGING_WARPS * (lane / UNIT_ROWS)) * UNIT_ROWS + lane % UNIT_ROWS : KEYS;
-    constexpr bool WHOLE = UNITS % STAGING_WARPS == 0;
-    auto mine = [&](int j) -> bool { return WHOLE || j < PIECES - 1 || w + STAGING_WARPS * j < UNITS; };      // the same for the warp
+    const int my_row = lane < PIECES * UNIT_ROWS ? (w + STAGING_WARPS * (lane / UNIT_ROWS)) * UNIT_ROWS + lane % UNIT_ROWS : KEYS;      // KEYS or more: none
+    auto mine = [&](int j) -> bool { return UNITS % STAGING_WARPS == 0 || j < PIECES - 1 || w + STAGING_WARPS * j < UNITS; };      // the same for the warp
     struct Row {
       long long at;                   // -1: not there
       int k_scale, v_scale;
@@ -274,8 +276,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
         const long long at = __shfl_sync(0xffffffffu, row.at, j * UNIT_ROWS + sub);
         if (mine(j))
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
-                       ::"r"(tc5::smem_u32(tile + code_offset((w + STAGING_WARPS * j) * UNIT_ROWS + sub, c))), "l"(p.k + (at < 0 ? 0 : at) * D + 16 * c),
-                         "r"(at < 0 ? 0 : 16));
+                     ::"r"(tc5::smem_u32(tile + code_offset((w + STAGING_WARPS * j) * UNIT_ROWS + sub, c))), "l"(p.k + (at < 0 ? 0 : at) * D + 16 * c),
+                       "r"(at < 0 ? 0 : 16));
       }
     };
     // a key whose value is not finite counts as not finite itself; missing ones are zero
@@ -332,31 +334,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
       if (lane == 0) arrive(bar);
     };
     // Links of a tile: its rows' pages, three tiles ahead; their places and scales and the keys' codes, two ahead; the
-    // values' codes, one ahead; the values as numbers.
+    // values' codes, one ahead; the values as numbers.  The loop starts two steps early instead of in front of itself: code
+    // that runs once costs the fetching of its instructions.
     uint4 values[PIECES];
-    int page0 = look_up(0), page1 = look_up(1), page = look_up(2);
-    Row now = find(page0, 0), next = find(page1, 1);
-    copy_keys(now, 0);
-    asm volatile("cp.async.commit_group;\n" ::);
-    copy_keys(next, 1);
-    asm volatile("cp.async.commit_group;\n" ::);
-    fetch_values(values, now);
-    put_factors(now, 0);
-    asm volatile("cp.async.wait_group 1;\n" ::: "memory");
-    publish(k_full);
-    for (int i = 0; i < steps; ++i) {
+    int page = look_up(0);
+    Row now = {-1, KV8_BIAS, KV8_BIAS}, next = now;
+#pragma unroll 1
+    for (int i = -2; i < steps; ++i) {
       const Row after = find(page, i + 2);
       page = look_up(i + 3);
-      if (i >= V_STAGES && !wait_event(i - V_STAGES + 1)) break;      // the value products of step i - 3 are done
-      store_values(values, now.v_scale == KV8_NAN ? KV8_BIAS : now.v_scale, i);
-      publish(v_full + i % V_STAGES);
-      fetch_values(values, next);
+      if (i >= 0) {
+        if (i >= V_STAGES && !wait_event(i - V_STAGES + 1)) break;      // the value products of step i - 3 are done
+        store_values(values, now.v_scale == KV8_NAN ? KV8_BIAS : now.v_scale, i);
+        publish(v_full + i % V_STAGES);
+      }
+      if (i >= -1) fetch_values(values, next);
       // the scores of step i - 1 are done, and the weights of step i - 2: nobody waits for an earlier phase of the
       // barriers that are arrived at below
       if (i >= 1 && !wait_event(i - 1)) break;
       if (i + 2 < steps) copy_keys(after, i + 2);
       asm volatile("cp.async.commit_group;\n" ::);
-      if (i + 1 < steps) {
+      if (i >= -1 && i + 1 < steps) {
         put_factors(next, i + 1);
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");       // the keys of step i + 1 are here
         publish(k_full + (i + 1) % K_STAGES);
@@ -365,68 +363,62 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
       next = after;
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-  } else if (warp == MMA_WARP) {
-    // ---- products ----
-    if (lane == 0) {
+  } else if (warp >= MMA_WARP) {
+    // ---- products of query tile x ----
+    const int x = warp - MMA_WARP;
+    if (lane == 0 && x < (t1.valid ? 2 : 1)) {
       const unsigned idesc_pv = tc5::umma_idesc(D) | (1u << 16);      // values: N-major
       const unsigned idesc_qk = 1u << 4 | (unsigned)(HALF >> 3) << 17 | (unsigned)(TILE_ROWS >> 4) << 24;      // e4m3 by e4m3, 32-bit sums
-      const uint64_t q_desc = desc_kmajor(q_tiles), k_desc = desc_kmajor(k_tiles), v_desc = desc_mnmajor(v_tiles, KEYS * 128);
-      auto scores = [&](int x, int i, int h) {
-        const uint64_t qa = q_desc + (uint64_t)(x * (2 * CODE_TILE >> 4));
+      const uint64_t q_desc = desc_kmajor(q_tiles + x * 2 * CODE_TILE), k_desc = desc_kmajor(k_tiles), v_desc = desc_mnmajor(v_tiles, KEYS * 128);
+      auto scores = [&](int i, int h) {
         const uint64_t kb = k_desc + (uint64_t)((i % K_STAGES) * (CODE_TILE >> 4) + h * (HALF * 128 >> 4));
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int kk = 0; kk < D / 32; ++kk)
-            mma_codes(tmem + COL_S + x * KEYS + h * HALF, qa + (uint64_t)(part * (CODE_TILE >> 4) + 2 * kk), kb + (uint64_t)(2 * kk), idesc_qk,
+            mma_codes(tmem + COL_S + x * KEYS + h * HALF, q_desc + (uint64_t)(part * (CODE_TILE >> 4) + 2 * kk), kb + (uint64_t)(2 * kk), idesc_qk,
                       (part | kk) != 0 ? 1u : 0u);
-        tc5::umma_commit(s_full + 2 * x + h);
       };
-      unsigned done[2] = {0u, 0u};
-      bool ok = wait(q_full, 0, abort_flag) && (!t1.valid || wait(q_full + 1, 0, abort_flag)) && wait(k_full, 0, abort_flag);
+      // 16 keys of an N-major tile: 2,048 bytes
+      auto products = [&](int i, int h, bool first) {
+        const uint64_t vb = v_desc + (uint64_t)((i % V_STAGES) * (V_BYTES >> 4) + h * (HALF * 128 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < HALF / 16; ++kk)
+          mma_ts(tmem + COL_O + x * 128, tmem + COL_S + x * KEYS + h * HALF + kk * 8, vb + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
+                 (first && kk == 0) ? 0u : 1u);
+      };
+      bool ok = wait(q_full + x, 0, abort_flag) && wait(k_full, 0, abort_flag);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (active(x, 0)) scores(x, 0, h);
+          if (active(x, 0)) {
+            scores(0, h);
+            tc5::umma_commit(s_full + 2 * x + h);
+          }
         tc5::umma_commit(freed);
       }
+      unsigned count = 0;
       for (int i = 0; i < steps && ok; ++i) {
-        const int s = i % V_STAGES;
-        const bool more = i + 1 < steps;
-        ok = wait(v_full + s, (i / V_STAGES) & 1, abort_flag);
-        if (ok && more) ok = wait(k_full + (i + 1) % K_STAGES, ((i + 1) / K_STAGES) & 1, abort_flag);
-        bool on[2], next[2];
+        const bool more = i + 1 < steps, on = active(x, i), next = more && active(x, i + 1);
+        // Both were asked for long ago.  A step without anything of x waits too, so that no event is arrived at before
+        // the one four earlier is over.
+        ok = wait(v_full + i % V_STAGES, (i / V_STAGES) & 1, abort_flag) &&
+             (!more || wait(k_full + (i + 1) % K_STAGES, ((i + 1) / K_STAGES) & 1, abort_flag));
 #pragma unroll
-        for (int x = 0; x < 2; ++x) { on[x] = active(x, i); next[x] = more && active(x, i + 1); }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (ok && on[x]) ok = wait(p_full + 2 * x + h, done[x] & 1, abort_flag);
-            if (!ok) break;
-            if (on[x]) {
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              const uint64_t vb = v_desc + (uint64_t)(s * (V_BYTES >> 4) + h * (HALF * 128 >> 4));
-#pragma unroll
-              for (int kk = 0; kk < HALF / 16; ++kk)          // 16 keys of an N-major tile: 2,048 bytes
-                mma_ts(tmem + COL_O + x * 128, tmem + COL_S + x * KEYS + h * HALF + kk * 8, vb + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
-                       (done[x] | h | kk) != 0 ? 1u : 0u);
-              tc5::umma_commit(pv_done + 2 * x + h);
-            }
-            // the scores of the next tile's half overwrite these weights: the tensor core runs them after the
-            // products above, while the softmax is at the other half
-            if (next[x]) scores(x, i + 1, h);
-          }
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (on) ok = wait(p_full + 2 * x + h, count & 1, abort_flag);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (on) products(i, h, count == 0 && h == 0);
+          // over the weights that the products read: the tensor core runs them afterwards
+          if (next) scores(i + 1, h);
+          if (on || next) tc5::umma_commit(s_full + 2 * x + h);
         }
-        if (!ok) break;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) done[x] += on[x] ? 1u : 0u;
-        if (more) tc5::umma_commit(freed + ((i + 1) & 3));
+        count += on ? 1u : 0u;
+        if (ok && more) tc5::umma_commit(freed + ((i + 1) & 3));
       }
-      tc5::umma_commit(o_full);
+      tc5::umma_commit(o_full + x);
     }
   } else {
     // ---- softmax: a thread a row of query tile x ----
@@ -440,51 +432,68 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
     const unsigned s_addr = lane_addr + COL_S + x * KEYS, o_addr = lane_addr + COL_O + x * 128;
     const int row_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
     const int tile_lo = p.window > 0 ? max(0, mine.pos_last - p.window + 1) : 0;        // first key all rows see
-    // The queries of this warp's 32 rows: D / 8 lanes take a row, a lane eight elements of it; all loads first.
-    constexpr int Q_LANES = D / 8, Q_ROWS = 32 / Q_LANES, Q_ROUNDS = 32 / Q_ROWS;
+    // The queries of this warp's 32 rows: D / 8 lanes take a row, a lane eight elements of it; four rounds' loads at a
+    // time, the next four on their way meanwhile.  In half precision, which holds a scaled row exactly but for what is
+    // below 2^-14, under the second part's steps of 2^-9.
+    constexpr int Q_LANES = D / 8, Q_ROWS = 32 / Q_LANES, Q_ROUNDS = 32 / Q_ROWS, BATCH = 4;
     float factor = 0.f;
     if (mine.valid) {
       const int c = lane % Q_LANES;
-      uint2 held[Q_ROUNDS][2];
+      // the rows of a lane are Q_ROWS apart; past the last one it stays
+      int from = mine.row0 + quarter * 32 + lane / Q_LANES;
+      const int token_step = Q_ROWS / p.groups, g_step = Q_ROWS - token_step * p.groups;
+      int token = min(from, rows - 1) / p.groups, g = min(from, rows - 1) - token * p.groups;
+      const bf16* base = p.q + (size_t)e.tok0 * p.q_stride + (size_t)kvh * p.groups * D + 8 * c;
+      uint2 held[BATCH][2];
+      auto load = [&]() {
 #pragma unroll
-      for (int n = 0; n < Q_ROUNDS; ++n) {
-        const int from = mine.row0 + quarter * 32 + n * Q_ROWS + lane / Q_LANES;
-        const int there = min(from, rows - 1), token = there / p.groups, g = there - token * p.groups;
-        const uint2* src = reinterpret_cast<const uint2*>(p.q + (size_t)(e.tok0 + token) * p.q_stride + (size_t)(kvh * p.groups + g) * D + 8 * c);
-        held[n][0] = src[0];                         // rows are multiples of four elements apart
-        held[n][1] = src[1];
-      }
-#pragma unroll
-      for (int n = 0; n < Q_ROUNDS; ++n) {
-        const int at = quarter * 32 + n * Q_ROWS + lane / Q_LANES;
-        float v[8];
-        load4(reinterpret_cast<const bf16*>(&held[n][0]), v);
-        load4(reinterpret_cast<const bf16*>(&held[n][1]), v + 4);
-        unsigned big = 0u;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = Q_LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const bool finite = big < 0x7f800000u;
-        const int ex = finite ? kv8_exponent(big) : 0;
-        const float down = __int_as_float((127 - ex) << 23);
-        unsigned hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = v[2 * k] * down, b = v[2 * k + 1] * down;
-          const unsigned short high = kv8_codes(a, b);
-          const unsigned h = kv8_half2(high);
-          const float2 rounded = __half22float2(*reinterpret_cast<const __half2*>(&h));
-          hi[k >> 1] |= (unsigned)high << (16 * (k & 1));
-          lo[k >> 1] |= (unsigned)kv8_codes(a - rounded.x, b - rounded.y) << (16 * (k & 1));
+        for (int n = 0; n < BATCH; ++n) {
+          const uint2* src = reinterpret_cast<const uint2*>(base + (size_t)token * p.q_stride + g * D);
+          held[n][0] = src[0];                         // rows are multiples of four elements apart
+          held[n][1] = src[1];
+          from += Q_ROWS;
+          if (from < rows) {
+            token += token_step;
+            g += g_step;
+            if (g >= p.groups) { g -= p.groups; ++token; }
+          }
         }
-        unsigned char* part = q_tiles + x * 2 * CODE_TILE + code_offset(at, c >> 1) + (c & 1) * 8;
-        *reinterpret_cast<uint2*>(part) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(part + CODE_TILE) = make_uint2(lo[0], lo[1]);
-        // what a score is multiplied by, in log2 units, goes to the lane whose row it is
-        const float up = finite ? p.scale_log2 * __int_as_float((127 + ex) << 23) : kv8_scale(KV8_NAN);
-        const float got = __shfl_sync(0xffffffffu, up, (lane % Q_ROWS) * Q_LANES);
-        if (lane / Q_ROWS == n) factor = got;
+      };
+      load();
+#pragma unroll 1
+      for (int n0 = 0; n0 < Q_ROUNDS; n0 += BATCH) {
+        unsigned here[BATCH][4];
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) { here[n][0] = held[n][0].x; here[n][1] = held[n][0].y; here[n][2] = held[n][1].x; here[n][3] = held[n][1].y; }
+        if (n0 + BATCH < Q_ROUNDS) load();
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+          const int at = quarter * 32 + (n0 + n) * Q_ROWS + lane / Q_LANES;
+          unsigned two = 0u;                           // largest |x| of both halves of the words, as bits
+#pragma unroll
+          for (int k = 0; k < 4; ++k) two = __vmaxu2(two, here[n][k] & 0x7fff7fffu);
+          unsigned big = max(two & 0xffff0000u, two << 16);
+#pragma unroll
+          for (int o = Q_LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const bool finite = big < 0x7f800000u;
+          const int ex = finite ? kv8_exponent(big) : 0;
+          const float down = __int_as_float((127 - ex) << 23);
+          unsigned hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __half2 v = __floats2half2_rn(__uint_as_float(here[n][k] << 16) * down, __uint_as_float(here[n][k] & 0xffff0000u) * down);
+            hi[k] = kv8_codes_of_half2(v);
+            const unsigned back = kv8_half2((unsigned short)hi[k]);
+            lo[k] = kv8_codes_of_half2(__hsub2(v, *reinterpret_cast<const __half2*>(&back)));
+          }
+          unsigned char* part = q_tiles + x * 2 * CODE_TILE + code_offset(at, c >> 1) + (c & 1) * 8;
+          *reinterpret_cast<uint2*>(part) = make_uint2(__byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
+          *reinterpret_cast<uint2*>(part + CODE_TILE) = make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
+          // what a score is multiplied by, in log2 units, goes to the lane whose row it is
+          const float up = finite ? p.scale_log2 * __int_as_float((127 + ex) << 23) : kv8_scale(KV8_NAN);
+          const float got = __shfl_sync(0xffffffffu, up, (lane % Q_ROWS) * Q_LANES);
+          if (lane / Q_ROWS == n0 + n) factor = got;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -492,14 +501,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
     }
     float m = -INFINITY, l = 0.f;
     bool ok = mine.valid;
-    unsigned count = 0;
+    unsigned count = 0;                // tiles of this query tile so far
+    // s_full[x][h] is arrived at by one commit before the first step, with its scores, and by one in every step that has
+    // products or the next step's scores of x, when both are done
+    unsigned commits = active(x, 0) ? 1u : 0u;
     for (int i = 0; i < steps && ok; ++i) {
-      if (!active(x, i)) continue;
-      // the keys' barrier too: what it published, their scales, is read here (its next phase needs these weights)
-      ok = wait(k_full + i % K_STAGES, (i / K_STAGES) & 1, abort_flag);
+      const bool on = active(x, i), next = i + 1 < steps && active(x, i + 1);
+      if (!on) {
+        commits += next ? 1u : 0u;
+        continue;
+      }
+      // the keys' barrier too: what it published, their scales, is read here (its next phase but one needs these weights)
+      ok = __all_sync(0xffffffffu, wait(k_full + i % K_STAGES, (i / K_STAGES) & 1, abort_flag));
 #pragma unroll 1
       for (int h = 0; h < 2 && ok; ++h) {
-        ok = wait(s_full + 2 * x + h, count & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, wait(s_full + 2 * x + h, (commits - 1) & 1, abort_flag));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int key0 = walk.tile(begin + i) * KEYS + h * HALF;
@@ -568,8 +584,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
         unpair(add2(sum_a, sum_b), sum0, sum1);
         l = l * corr + (sum0 + sum1);
         if ((count > 0 || h > 0) && __any_sync(0xffffffffu, corr != 1.f)) {
-          // the value products so far have to be done: the other half's last ones
-          ok = wait(pv_done + 2 * x + (h ^ 1), (h ? count : count - 1) & 1, abort_flag);
+          // the value products so far have to be done: the first half's of this step, or the second half's of the step
+          // before, which the scores of this step's second half came with
+          ok = __all_sync(0xffffffffu, wait(s_full + 2 * x + (h ^ 1), (h ? commits : commits - 1) & 1, abort_flag));
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -588,32 +605,47 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
         if (lane == 0) arrive(p_full + 2 * x + h);
       }
       ++count;
+      ++commits;
     }
-    if (ok) ok = wait(o_full, 0, abort_flag);
+    if (ok) ok = __all_sync(0xffffffffu, wait(o_full + x, 0, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int token = row / p.groups, g = row - token * p.groups;
-      bf16* dst = p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D;
       const int ur = x * TILE_ROWS + r;
+      const float by = pieces > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       float* ws = p.ws + ((((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans + piece) * (size_t)PORTION_UNIT * (D + 2);
+      // a finished warp's 32 rows pass through its queries' place, so that whole rows go out
+      unsigned char* rows_here = q_tiles + x * 2 * CODE_TILE + quarter * 32 * D * 2;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 64) {
-        unsigned raw[64];
+      for (int c = 0; c < D; c += 32) {
+        unsigned raw[32];
         tmem_ld32(o_addr + c, raw);
-        tmem_ld32(o_addr + c + 32, raw + 32);
         tmem_wait_ld();
-        if (!row_valid) continue;
 #pragma unroll
-        for (int j = 0; j < 64; j += 8) {
+        for (int j = 0; j < 32; j += 8) {
           float o[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = count == 0 ? 0.f : __uint_as_float(raw[j + k]) * (pieces == 1 ? inv : 1.f);      // no key: nothing was summed
-          if (pieces == 1) store8(dst + c + j, o);
-          else store8(ws + piece_element<PORTION_UNIT>(ur, c + j), o);
+          for (int k = 0; k < 8; ++k) o[k] = count == 0 ? 0.f : __uint_as_float(raw[j + k]) * by;      // no key of this piece: nothing was summed
+          if (pieces == 1) {
+            const int chunk = (c + j) >> 3;
+            store8(reinterpret_cast<bf16*>(rows_here + lane * D * 2 + ((chunk ^ (lane & 7)) << 4)), o);
+          } else if (row_valid) {
+            store8(ws + piece_element<PORTION_UNIT>(ur, c + j), o);
+          }
         }
       }
-      if (pieces > 1 && row_valid) {
+      if (pieces == 1) {
+        __syncwarp();
+        constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+        const int chunk = lane % LANES;
+#pragma unroll 4
+        for (int n = lane / LANES; n < 32; n += AT_ONCE) {
+          const int out_row = mine.row0 + quarter * 32 + n;
+          if (out_row >= rows) break;
+          const int token = out_row / p.groups, g = out_row - token * p.groups;
+          *reinterpret_cast<uint4*>(p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D + 8 * chunk) =
+              *reinterpret_cast<const uint4*>(rows_here + n * D * 2 + ((chunk ^ (n & 7)) << 4));
+        }
+      } else if (row_valid) {
         ws[(size_t)PORTION_UNIT * D + 2 * ur] = m;
         ws[(size_t)PORTION_UNIT * D + 2 * ur + 1] = l;
       }

@@ -14,6 +14,8 @@
 // back as NaN, a query that sees it gets NaN, and a query that does not see it is not reached, because
 // masked scores are replaced and a zero weight times a zero code is zero.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "attention_common.cuh"
 
 constexpr int KV8_LEAST = -64, KV8_MOST = 64;     // bounds of e
@@ -35,6 +37,13 @@ __device__ __forceinline__ int kv8_exponent(unsigned bits) {
 __device__ __forceinline__ unsigned short kv8_codes(float lo, float hi) {
   unsigned short r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// the same of two half-precision numbers
+__device__ __forceinline__ unsigned kv8_codes_of_half2(__half2 v) {
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const unsigned*>(&v)));
   return r;
 }
 
