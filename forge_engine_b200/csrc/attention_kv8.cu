@@ -30,22 +30,20 @@ using namespace kv8;
 namespace {
 
 constexpr int CHUNKS = D / 16;          // 16-byte pieces of a cached vector
-constexpr int KEYS = 64;                // keys of a tile
+constexpr int KEYS = 128;               // keys of a tile
+constexpr int STEP = 32;                // keys a warp takes at a time
 constexpr int ROWS = 16;                // rows a warp takes: the m of one mma
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int STAGES = D <= 128 ? 4 : 3;
-constexpr int MATRIX = KEYS * D;        // bytes of one matrix of a stage
-constexpr int STAGE = 2 * MATRIX + 2 * KEYS;
-constexpr size_t MMA_SMEM_RING = (size_t)STAGES * STAGE;
-constexpr size_t MMA_SMEM_JOIN = (size_t)WARPS * ROWS * (D + 2) * sizeof(float);
-constexpr size_t MMA_SMEM = MMA_SMEM_RING > MMA_SMEM_JOIN ? MMA_SMEM_RING : MMA_SMEM_JOIN;
+constexpr int STAGES = 2;
+constexpr int MATRIX = STEP * D;        // bytes of one matrix of a stage
+constexpr int STAGE = 2 * MATRIX + 3 * STEP * 4;      // codes, then of every key: 2^a, b and 2^-b
+constexpr size_t RING = (size_t)WARPS * STAGES * STAGE;
+constexpr size_t JOIN = (size_t)WARPS * ROWS * (D + 2) * sizeof(float);
+constexpr size_t MMA_SMEM = RING > JOIN ? RING : JOIN;
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0));
-}
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 4 : 0));
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
@@ -53,6 +51,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], u
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {       // the weight is rounded to 11 bits anyway
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -66,52 +69,6 @@ __device__ __forceinline__ int key_piece(int r, int c) { return D % 128 == 0 ? c
 __device__ __forceinline__ int value_piece(int r, int c) {
   return D % 128 == 0 ? c ^ (((r >> 1) & 3) << 1) : D % 64 == 0 ? c ^ ((r >> 1) & 3) : c;
 }
-
-// Stages tiles of 64 keys of one kv head, their values and both scales.  What lies at or past key_end is zero.  A
-// thread copies 16-byte pieces of up to COPIES rows; the rows' pages are looked up a tile ahead.
-struct Staging {
-  static constexpr int COPIES = (KEYS * CHUNKS + THREADS - 1) / THREADS;
-  int pages[COPIES], scale_page;
-
-  static __device__ __forceinline__ int scale_row(const Kv8Attention& p, int tid) {
-    return p.page_size % 4 == 0 ? (tid % (KEYS / 4)) * 4 : tid % KEYS;
-  }
-
-  __device__ __forceinline__ void look_up(const Kv8Attention& p, const int* table, int key0, int key_end, int tid) {
-#pragma unroll
-    for (int j = 0; j < COPIES; ++j) {
-      const int row = (tid + j * THREADS) / CHUNKS;
-      pages[j] = row < KEYS ? key_page(p, table, key0 + row, key_end) : -1;
-    }
-    scale_page = key_page(p, table, key0 + scale_row(p, tid), key_end);
-  }
-
-  __device__ __forceinline__ void copy(unsigned char* stage, const Kv8Attention& p, int kvh, int key0, int key_lo, int key_end, int tid) const {
-    unsigned char* kd = stage;
-    unsigned char* vd = stage + MATRIX;
-    unsigned char* sd = stage + 2 * MATRIX;
-#pragma unroll
-    for (int j = 0; j < COPIES; ++j) {
-      const int u = tid + j * THREADS, row = u / CHUNKS, c = u - row * CHUNKS;
-      if (KEYS * CHUNKS % THREADS != 0 && row >= KEYS) break;
-      long long at;
-      const bool there = key_row(p, pages[j], kvh, key0 + row, &at);
-      if (!there && c == 0) tell_missing(p, key0 + row, key_lo, key_end);
-      cp_async16(kd + row * D + key_piece(row, c) * 16, p.k + at * D + c * 16, there);
-      cp_async16(vd + row * D + value_piece(row, c) * 16, p.v + at * D + c * 16, there);
-    }
-    const int row = scale_row(p, tid);
-    long long at;
-    const bool there = key_row(p, scale_page, kvh, key0 + row, &at);
-    if (p.page_size % 4 == 0) {          // four neighbouring scales lie in one word
-      const int m = tid / (KEYS / 4);
-      if (m < 2) cp_async4(sd + m * KEYS + row, (m ? p.vs : p.ks) + at, there);
-    } else {
-      const int m = tid / KEYS;
-      sd[m * KEYS + row] = there ? (m ? p.vs : p.ks)[at] : 0;
-    }
-  }
-};
 
 // The queries of a warp's 16 rows as the A operand.  The order of the contraction is free as long as both
 // operands keep it: in every stretch of 64 elements lane t of a quad holds elements 16 t .. 16 t + 15, which it
@@ -223,62 +180,51 @@ __device__ __forceinline__ int value_column(int n, int c, int t) {
   return base + 2 * (2 * t + c) + (n * 8 - base) / 8;
 }
 
-// 16 keys (k0 .. k0 + 15 of the staged tile, positions from key0 on) against a warp's 16 rows.
-__device__ __forceinline__ void step16(const Queries& q, const unsigned char* stage, int k0, int key0, const Kv8Attention& p,
-                                       bool clear, int pos_a, int pos_b, Sums& s, int lane) {
+// The 32 keys of a stage, at positions from key0 on, against a warp's 16 rows.
+__device__ __forceinline__ void take(const Queries& q, const unsigned char* stage, int key0, const Kv8Attention& p, bool clear,
+                                     int pos_a, int pos_b, Sums& s, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  const unsigned char* ks = stage;
-  const unsigned char* scales = stage + 2 * MATRIX;
-  float c[2][4];
+  const float* of_key = reinterpret_cast<const float*>(stage + 2 * MATRIX);
+  float c[STEP / 8][4];
+  float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < STEP / 8; ++n) {
     c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-    const int row = k0 + 8 * n + g;
+    const int row = 8 * n + g;
     unsigned w[D / 16];
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint4 x = *reinterpret_cast<const uint4*>(ks + row * D + key_piece(row, 4 * b + t) * 16);
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + row * D + key_piece(row, 4 * b + t) * 16);
       w[4 * b] = x.x; w[4 * b + 1] = x.y; w[4 * b + 2] = x.z; w[4 * b + 3] = x.w;
     }
     if constexpr ((D & 32) != 0) {
-      const uint2 x = *reinterpret_cast<const uint2*>(ks + row * D + D / 64 * 64 + 8 * t);
+      const uint2 x = *reinterpret_cast<const uint2*>(stage + row * D + D / 64 * 64 + 8 * t);
       w[D / 64 * 4] = x.x; w[D / 64 * 4 + 1] = x.y;
     }
-    if constexpr ((D & 16) != 0) w[D / 16 - 1] = *reinterpret_cast<const unsigned*>(ks + row * D + D - 16 + 4 * t);
+    if constexpr ((D & 16) != 0) w[D / 16 - 1] = *reinterpret_cast<const unsigned*>(stage + row * D + D - 16 + 4 * t);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
       mma_f16(c[n], q.a[i], kv8_half2((unsigned short)w[i]), kv8_half2((unsigned short)(w[i] >> 16)));
-  }
-  // keys k0 + 8 n + 2 t + i: factor of the score, exponent and reciprocal scale of the value
-  float mx[2] = {-INFINITY, -INFINITY};
-  float back[2][2];
+    // keys 8 n + 2 t and the next one
+    const float2 up = *reinterpret_cast<const float2*>(of_key + 8 * n + 2 * t);
+    const float2 add = *reinterpret_cast<const float2*>(of_key + STEP + 8 * n + 2 * t);
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int at = k0 + 8 * n + 2 * t;
-    const unsigned kb = *reinterpret_cast<const unsigned short*>(scales + at);
-    const unsigned vb = *reinterpret_cast<const unsigned short*>(scales + KEYS + at);
+    for (int h = 0; h < 2; ++h) {
+      c[n][2 * h] = fmaf(c[n][2 * h] * up.x, q.factor[h], add.x);
+      c[n][2 * h + 1] = fmaf(c[n][2 * h + 1] * up.y, q.factor[h], add.y);
+    }
+    if (!clear) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int a = (kb >> (8 * i)) & 255, b = (vb >> (8 * i)) & 255;
-      const float up = b == KV8_NAN ? kv8_scale(KV8_NAN) : kv8_scale(a);
-      const float add = b == KV8_NAN ? 0.f : (float)(b - KV8_BIAS);
-      back[n][i] = b == KV8_NAN ? 1.f : __int_as_float((254 - b) << 23);
-      const int key = key0 + 8 * n + 2 * t + i;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float u = c[n][2 * h + i] * up * q.factor[h] + add;
-        if (!clear) {
-          const int pos = h ? pos_b : pos_a;
-          const bool seen = key <= pos && (p.window <= 0 || pos - key < p.window || key < p.keep_first);
-          if (!seen) u = -INFINITY;
-        }
-        c[n][2 * h + i] = u;
-        mx[h] = fmaxf(mx[h], u);
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 8 * n + 2 * t + (e & 1), pos = e < 2 ? pos_a : pos_b;
+        const bool seen = key <= pos && (p.window <= 0 || pos - key < p.window || key < p.keep_first);
+        if (!seen) c[n][e] = -INFINITY;
       }
     }
+    mx[0] = fmaxf(mx[0], fmaxf(c[n][0], c[n][1]));
+    mx[1] = fmaxf(mx[1], fmaxf(c[n][2], c[n][3]));
   }
   float corr[2], base[2], sum[2] = {0.f, 0.f};
-  unsigned a[4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
@@ -288,32 +234,39 @@ __device__ __forceinline__ void step16(const Queries& q, const unsigned char* st
     s.m[h] = now;
     base[h] = now == -INFINITY ? 0.f : now;
   }
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float w0 = exp2f(c[n][2 * h] - base[h]), w1 = exp2f(c[n][2 * h + 1] - base[h]);
-      sum[h] += w0 * back[n][0] + w1 * back[n][1];
-      a[2 * n + h] = pack_half(w0, w1);
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) s.l[h] = s.l[h] * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
   if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) { s.o[n][0] *= corr[0]; s.o[n][1] *= corr[0]; s.o[n][2] *= corr[1]; s.o[n][3] *= corr[1]; }
   }
-  const unsigned char* vs = stage + MATRIX;
-  value_stretch<0, D >= 128 ? 16 : D >= 64 ? 8 : D >= 32 ? 4 : 2>(vs, k0, a, s.o, lane);
-  if constexpr (D == 256) value_stretch<128, 16>(vs, k0, a, s.o, lane);
-  if constexpr (D > 128 && D < 256 && (D & 64) != 0) value_stretch<128, 8>(vs, k0, a, s.o, lane);
-  if constexpr (D > 64 && (D & 32) != 0) value_stretch<D / 64 * 64, 4>(vs, k0, a, s.o, lane);
-  if constexpr (D > 16 && (D & 16) != 0) value_stretch<D / 32 * 32, 2>(vs, k0, a, s.o, lane);
+#pragma unroll
+  for (int k = 0; k < STEP / 16; ++k) {
+    unsigned a[4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const float2 back = *reinterpret_cast<const float2*>(of_key + 2 * STEP + 16 * k + 8 * n + 2 * t);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float w0 = exp2_fast(c[2 * k + n][2 * h] - base[h]), w1 = exp2_fast(c[2 * k + n][2 * h + 1] - base[h]);
+        sum[h] = fmaf(w0, back.x, fmaf(w1, back.y, sum[h]));
+        a[2 * n + h] = pack_half(w0, w1);
+      }
+    }
+    const unsigned char* vs = stage + MATRIX;
+    value_stretch<0, D >= 128 ? 16 : D >= 64 ? 8 : D >= 32 ? 4 : 2>(vs, 16 * k, a, s.o, lane);
+    if constexpr (D == 256) value_stretch<128, 16>(vs, 16 * k, a, s.o, lane);
+    if constexpr (D > 128 && D < 256 && (D & 64) != 0) value_stretch<128, 8>(vs, 16 * k, a, s.o, lane);
+    if constexpr (D > 64 && (D & 32) != 0) value_stretch<D / 64 * 64, 4>(vs, 16 * k, a, s.o, lane);
+    if constexpr (D > 16 && (D & 16) != 0) value_stretch<D / 32 * 32, 2>(vs, 16 * k, a, s.o, lane);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) s.l[h] = s.l[h] * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
 }
 
-// PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of a tile.  Otherwise it takes the (at most
-// 16) rows of an entry, and warp w the keys 16 w .. 16 w + 15 of every tile; the warps' sums join at the end.
-// Key tiles come through a ring of STAGES by asynchronous copies, a page looked up per row.
+// PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of its tiles.  Otherwise it takes the (at most
+// 16) rows of an entry, and warp w the keys 32 w .. 32 w + 31 of every tile; the warps' sums join at the end.
+// A warp goes its own way: it copies its keys into a ring of its own, a step ahead, and waits for nobody (with a ring of the
+// block and a barrier a tile, 64 keys of one head took 1.7 us a block whatever else ran).  A lane looks after one key: its
+// page, two steps ahead, its place and its scales.
 // grid: (spans x row tiles, entries, kv heads); a block takes `span` key tiles of its unit.
 template <bool PORTION>
 __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
@@ -333,46 +286,71 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   const int pieces = pieces_of(p, walk.count);
   if (piece >= pieces) return;
   const int begin = piece * p.span, end = piece == pieces - 1 ? walk.count : begin + p.span;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int* table = p.block_table + (size_t)entry * p.max_pages;
+  unsigned char* ring = smem + warp * (STAGES * STAGE);
+  const int steps = (end - begin) * (PORTION ? KEYS / STEP : 1);
+  auto key0_of = [&](int i) -> int {
+    return PORTION ? walk.tile(begin + i / (KEYS / STEP)) * KEYS + i % (KEYS / STEP) * STEP : walk.tile(begin + i) * KEYS + warp * STEP;
+  };
+  auto look_up = [&](int i) -> int { return i < steps ? key_page(p, table, key0_of(i) + lane, walk.key_end) : -1; };
 
-  auto key0_of = [&](int i) -> int { return walk.tile(i) * KEYS; };
-  Staging staging[STAGES - 1];           // all lookups of the first tiles at once
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) staging[i].look_up(p, table, key0_of(min(begin + i, end - 1)), walk.key_end, tid);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (begin + i < end) staging[i].copy(smem + i * STAGE, p, kvh, key0_of(begin + i), walk.key_lo, walk.key_end, tid);
-    cp_async_commit();
-  }
-  Staging& next = staging[0];
-  next.look_up(p, table, key0_of(min(begin + STAGES - 1, end - 1)), walk.key_end, tid);
   const int wrow0 = PORTION ? row0 + warp * ROWS : row0;
-  Queries q;
-  q.load(p, e, kvh, wrow0, rows_end, lane);
   // rows past the end take the last row's position; nobody reads them
   const int last = rows_end - 1;
   const int pos_a = e.start + min(wrow0 + g, last) / p.groups, pos_b = e.start + min(wrow0 + g + 8, last) / p.groups;
   const int pos_min = e.start + min(wrow0, last) / p.groups, pos_max = e.start + min(wrow0 + ROWS - 1, last) / p.groups;
+  Queries q;
   Sums s;
   s.clear();
-  for (int i = begin; i < end; ++i) {
-    cp_async_wait<STAGES - 2>();
-    __syncthreads();                 // the tile is here, and the stage filled next is no longer read
-    const int ahead = i + STAGES - 1;
-    if (ahead < end) next.copy(smem + ((ahead - begin) % STAGES) * STAGE, p, kvh, key0_of(ahead), walk.key_lo, walk.key_end, tid);
-    cp_async_commit();
-    if (ahead + 1 < end) next.look_up(p, table, key0_of(ahead + 1), walk.key_end, tid);
-    const unsigned char* stage = smem + ((i - begin) % STAGES) * STAGE;
-    const int key0 = walk.tile(i) * KEYS;
-    for (int j = PORTION ? 0 : warp; j < (PORTION ? KEYS / 16 : warp + 1); ++j) {
-      const int first = key0 + 16 * j;
-      if (first > pos_max) continue;
-      const bool clear = first + 15 <= pos_min && (p.window <= 0 || pos_max - first < p.window);
-      step16(q, stage, 16 * j, first, p, clear, pos_a, pos_b, s, lane);
+  int page = look_up(0);
+  int k_scale = KV8_BIAS, v_scale = KV8_BIAS;       // of this lane's key of the step whose copies were asked for last
+#pragma unroll 1
+  for (int i = -1; i < steps; ++i) {
+    if (i >= 0) {
+      // the scales of step i, asked for with its copies; a key whose value is not finite counts as not finite itself
+      float* of_key = reinterpret_cast<float*>(ring + (i & 1) * STAGE + 2 * MATRIX);
+      const bool bad = v_scale == KV8_NAN;
+      of_key[lane] = kv8_scale(bad ? KV8_NAN : k_scale);
+      of_key[STEP + lane] = bad ? 0.f : (float)(v_scale - KV8_BIAS);
+      of_key[2 * STEP + lane] = bad ? 1.f : __int_as_float((2 * KV8_BIAS - v_scale) << 23);
     }
+    if (i + 1 < steps) {
+      const int key = key0_of(i + 1) + lane;
+      long long at;
+      const bool there = key_row(p, page, kvh, key, &at);
+      if (!there) tell_missing(p, key, walk.key_lo, walk.key_end);
+      k_scale = v_scale = KV8_BIAS;
+      if (there) {
+        k_scale = __ldg(p.ks + at);
+        v_scale = __ldg(p.vs + at);
+      }
+      page = look_up(i + 2);
+      const int mine = there ? (int)at : -1;             // the launcher holds the rows of a cache to 31 bits
+      unsigned char* stage = ring + ((i + 1) & 1) * STAGE;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        const int u = lane + 32 * j, row = u / CHUNKS, c = u - row * CHUNKS;
+        const int from = __shfl_sync(0xffffffffu, mine, row);
+        const size_t offset = (size_t)max(from, 0) * D + c * 16;
+        cp_async16(stage + row * D + key_piece(row, c) * 16, p.k + offset, from >= 0);
+        cp_async16(stage + MATRIX + row * D + value_piece(row, c) * 16, p.v + offset, from >= 0);
+      }
+    }
+    cp_async_commit();
+    if (i < 0) {
+      q.load(p, e, kvh, wrow0, rows_end, lane);
+      continue;
+    }
+    cp_async_wait<1>();
+    __syncwarp();
+    const int key0 = key0_of(i);
+    if (key0 <= pos_max) {
+      const bool clear = key0 + STEP - 1 <= pos_min && (p.window <= 0 || pos_max - key0 < p.window);
+      take(q, ring + (i & 1) * STAGE, key0, p, clear, pos_a, pos_b, s, lane);
+    }
+    __syncwarp();
   }
-  cp_async_wait<0>();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);
@@ -384,7 +362,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
     for (int h = 0; h < 2; ++h) {
       const int r = warp * ROWS + g + 8 * h, row = row0 + r;
       if (row >= rows_end) continue;
-      const float inv = s.l[h] > 0.f ? 1.f / s.l[h] : (s.l[h] == 0.f ? 0.f : s.l[h]);
+      const float inv = s.l[h] == 0.f ? 0.f : 1.f / s.l[h];
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -399,40 +377,53 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
       }
     }
   } else {
-    __syncthreads();                 // the ring's space takes the warps' sums
+    const int n_rows = rows_end - row0;
+    __syncthreads();                 // the rings' space takes the warps' sums
     float* acc = reinterpret_cast<float*>(smem);           // [WARPS][16][D]
     float* ml = acc + WARPS * ROWS * D;                    // [WARPS][16][2]
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = g + 8 * h;
-      if (row0 + r >= rows_end) continue;
+      if (r >= n_rows) continue;
+      float* to = acc + (warp * ROWS + r) * D;
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
+      for (int n = 0; n < D / 8; n += (D % 32 == 0 ? 4 : 1))
 #pragma unroll
-        for (int c = 0; c < 2; ++c) acc[(warp * ROWS + r) * D + value_column(n, c, t)] = s.o[n][2 * h + c];
+        for (int c = 0; c < 2; ++c) {
+          // in stretches of 32 columns and more, four n-tiles are four neighbouring columns
+          if constexpr (D % 32 == 0)
+            *reinterpret_cast<float4*>(to + value_column(n, c, t)) = make_float4(s.o[n][2 * h + c], s.o[n + 1][2 * h + c], s.o[n + 2][2 * h + c], s.o[n + 3][2 * h + c]);
+          else
+            to[value_column(n, c, t)] = s.o[n][2 * h + c];
+        }
       if (t == 0) {
         ml[(warp * ROWS + r) * 2] = s.m[h];
         ml[(warp * ROWS + r) * 2 + 1] = s.l[h];
       }
     }
     __syncthreads();
-    for (int i = tid; i < (rows_end - row0) * D; i += THREADS) {
-      const int r = i / D, d = i - r * D;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n_rows * (D / 4); i += THREADS) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
       float big = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) big = fmaxf(big, ml[(w * ROWS + r) * 2]);
-      float num = 0.f, den = 0.f;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float mw = ml[(w * ROWS + r) * 2], lw = ml[(w * ROWS + r) * 2 + 1];
-        const float f = piece_share(mw, lw, big);
-        num += acc[(w * ROWS + r) * D + d] * f;
-        den += lw * f;
+        const float f = piece_share(ml[(w * ROWS + r) * 2], ml[(w * ROWS + r) * 2 + 1], big);
+        const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROWS + r) * D + d);
+        num.x += x.x * f; num.y += x.y * f; num.z += x.z * f; num.w += x.w * f;
+        den += ml[(w * ROWS + r) * 2 + 1] * f;
       }
       if (pieces == 1) {
-        store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : num / den);
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const float out[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+        const int row = row0 + r, token = row / p.groups, gq = row - token * p.groups;
+        store4(p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + gq) * D + d, out);
       } else {
-        ws[piece_element<UNIT>(r, d)] = num;
+        *reinterpret_cast<float4*>(ws + piece_element<UNIT>(r, d)) = num;
         if (d == 0) { ws[(size_t)UNIT * D + 2 * r] = big; ws[(size_t)UNIT * D + 2 * r + 1] = den; }
       }
     }
@@ -470,8 +461,7 @@ FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, 
 }
 
 // The entries of a step with at most 16 rows (new tokens x heads per kv head) if single_spans is above zero, the others
-// if portion_spans is; `*_span` key tiles a block (of 64 keys, of 128 in the tcgen05 kernel of portions), `*_spans` of
-// them for the longest.
+// if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
                                       int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new,
@@ -482,6 +472,7 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
   if (single_spans < 0 || portion_spans < 0 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
   if ((single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
+  if ((long long)num_pages * nkv > 0x7fffffffLL / page_size) return FE_ERR_TOO_LARGE;       // rows of a cache: 31 bits
   if (entries > 65535 || nkv > 65535 || (long long)max_new * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
   if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) ||
       q_stride % 4)

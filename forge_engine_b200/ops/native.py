@@ -1891,7 +1891,7 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor, status: torch.Tensor, w
 
 KV8_CODES, KV8_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_SINGLE_ROWS = 16         # rows (new tokens x heads per kv head) of an entry that the kernel of single tokens takes
-KV8_TILE = 64                # keys of a tile
+KV8_TILE = 128               # keys of a tile
 KV8_TC5_DIMS = (64, 128)     # head sizes whose portions the tcgen05 kernel takes
 
 _kv8_handles: dict = {}
@@ -2049,7 +2049,7 @@ def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, 
 
 @_functools.lru_cache(maxsize=4096)
 def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int, keep_first: int) -> tuple:
-    rows_of, tile, slots = (256, 128, 148) if head_dim in KV8_TC5_DIMS else (64, KV8_TILE, 296)
+    rows_of, slots = (256, 148) if head_dim in KV8_TC5_DIMS else (64, 296)
     single, portion = [], []
     for start, count in entries:
         rows = count * groups
@@ -2057,7 +2057,7 @@ def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int,
             single.append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
         elif rows:
             for row in range(0, rows, rows_of):
-                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, tile))
+                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
     return (*_kv8_cut(single, nkv, 444, 2.0, 4.0), *_kv8_cut(portion, nkv, slots, 3.0, 4.0))
 
 

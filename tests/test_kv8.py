@@ -123,5 +123,4 @@ def test_plans_cover_every_key(entries, window, keep) -> None:
         for (start, n), r in zip(entries, rows):
             if r and not window:
                 span, spans = (single_span, single_spans) if r <= 16 else (portion_span, portion_spans)
-                tile = 128 if r > 16 and dim in native.KV8_TC5_DIMS else native.KV8_TILE
-                assert span >= 1 and spans >= 1 and (spans & (spans - 1)) == 0 and span * spans * tile >= start + n
+                assert span >= 1 and spans >= 1 and (spans & (spans - 1)) == 0 and span * spans * native.KV8_TILE >= start + n
