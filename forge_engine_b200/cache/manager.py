@@ -27,7 +27,8 @@ class PagedKVSpec:
     ``v_head_dim``: size of a value head where it differs (None: ``head_dim``; 0: the run
     keeps one vector per token and head, no second one - a latent that is key and value).
     ``keep_first``: with a window, positions below it stay visible for ever, so the pages
-    that hold them are never given back.  ``chunk`` (not together with a window): a token sees
+    that hold them are never given back.  ``eight_bit``: the run reads and writes an 8-bit cache
+    (``ops.native.kv8_write``): e4m3 codes and a power-of-two scale per token, head and matrix.  ``chunk`` (not together with a window): a token sees
     its own chunk of that many positions only, counted from position 0."""
 
     num_kv_heads: int
@@ -36,6 +37,7 @@ class PagedKVSpec:
     v_head_dim: int | None = None
     keep_first: int = 0
     chunk: int | None = None
+    eight_bit: bool = False
 
     def kept_pages(self, page_size: int) -> int:
         """Leading pages a window never releases."""
@@ -89,8 +91,10 @@ class LayerGroup:
     units: list  # run indices that own a cache in this group
     pool: PagePool
     # [units, 2, pages, kv_heads, page_size, head_dim]; where values have another size than
-    # keys, one flat tensor: per unit all key pages, then all value pages
+    # keys, one flat tensor: per unit all key pages, then all value pages.  An 8-bit cache: its codes
     storage: object = None
+    # scales of an 8-bit cache [units, 2, pages, kv_heads, page_size]
+    scales: object = None
 
     def unit_slot(self, run: int) -> int:
         return self.units.index(run)
@@ -183,6 +187,21 @@ class CacheManager:
         import torch
 
         self.guarded = []
+
+        def pool(name: str, shape: tuple, dtype):
+            numel = 1
+            for extent in shape:
+                numel *= extent
+            if torch.device(self.device).type != "cuda":
+                return torch.zeros(shape, dtype=dtype, device=self.device)
+            # canary words before and after the pool: a write to "page -1" or past the
+            # last page shows in ``native.damaged_canaries(cache.guarded)``
+            from ..ops.native import GuardedBuffer
+
+            buffer = GuardedBuffer(name, numel, dtype, self.device, zero=True)
+            self.guarded.append(buffer)
+            return buffer.data.view(shape)
+
         for group in self.groups:
             spec = group.spec
             # one page more than the pool leases: ``null_page`` takes the keys of filler
@@ -191,19 +210,14 @@ class CacheManager:
             if spec.value_dim != spec.head_dim:
                 rows = (self.num_pages + 1) * spec.num_kv_heads * self.page_size
                 shape = (len(group.units) * rows * (spec.head_dim + spec.value_dim),)
-            numel = 1
-            for extent in shape:
-                numel *= extent
-            if torch.device(self.device).type == "cuda":
-                # canary words before and after the pool: a write to "page -1" or past the
-                # last page shows in ``native.damaged_canaries(cache.guarded)``
-                from ..ops.native import GuardedBuffer
-
-                buffer = GuardedBuffer(f"cache pool of layer group {group.index}", numel, self.dtype, self.device, zero=True)
-                self.guarded.append(buffer)
-                group.storage = buffer.data.view(shape)
+            name = f"cache pool of layer group {group.index}"
+            if spec.eight_bit:
+                if spec.value_dim != spec.head_dim:
+                    raise ValueError("an 8-bit cache has keys and values of one size")
+                group.storage = pool(name, shape, torch.uint8).view(torch.float8_e4m3fn)
+                group.scales = pool(f"scales of layer group {group.index}", shape[:-1], torch.uint8).view(torch.float8_e8m0fnu)
             else:
-                group.storage = torch.zeros(shape, dtype=self.dtype, device=self.device)
+                group.storage = pool(name, shape, self.dtype)
         for run, spec in self._state_specs.items():
             self._run_state[run] = torch.zeros(
                 (self.max_requests + 1, *spec.shape), dtype=getattr(torch, spec.dtype), device=self.device
@@ -224,7 +238,9 @@ class CacheManager:
 
         size = torch.empty((), dtype=self.dtype).element_size() if self.dtype is not None else 2
         return sum(
-            len(g.units) * g.spec.num_kv_heads * (g.spec.head_dim + g.spec.value_dim) * size for g in self.groups
+            len(g.units) * g.spec.num_kv_heads
+            * (2 * (g.spec.head_dim + 1) if g.spec.eight_bit else (g.spec.head_dim + g.spec.value_dim) * size)
+            for g in self.groups
         )
 
     def group_of_run(self, run: int) -> int | None:
@@ -248,6 +264,43 @@ class CacheManager:
         begin += rows * spec.head_dim
         return keys, storage[begin : begin + rows * spec.value_dim].view(*lead, spec.value_dim)
 
+    def scales_of_run(self, run: int) -> tuple | None:
+        """(scales of the keys, of the values) [pages, kv_heads, page_size] of a run with an 8-bit cache."""
+        group_index, unit = self._run_group[run]
+        scales = self.groups[group_index].scales
+        return None if scales is None else (scales[unit, 0], scales[unit, 1])
+
+    def read(self, key, run: int, first: int = 0, count: int | None = None, dtype=None) -> tuple:
+        """Keys and values [count, kv_heads, head_dim] that request ``key`` holds at positions ``first`` .. of run ``run``
+        (to its end where ``count`` is None), in ``dtype`` (the cache's; of an 8-bit cache the engine's): a copy, for
+        looking at a cache or handing it on.  Positions whose pages a window has given back are refused."""
+        import torch
+
+        entry = self.request(key)
+        group_index, _ = self._run_group[run]
+        spec, table = self.groups[group_index].spec, entry.tables[group_index]
+        count = entry.length - first if count is None else count
+        if first < 0 or count < 0 or first + count > entry.length:
+            raise ValueError(f"request {key!r} holds {entry.length} positions, not {first} to {first + count}")
+        if spec.value_dim == 0:
+            raise ValueError("the run keeps one vector a token, not keys and values")
+        k_cache, v_cache = self.kv_of_run(run)
+        places = [table.pages[at // self.page_size] for at in range(first, first + count)]
+        if any(page < 0 for page in places):
+            raise ValueError(f"request {key!r}: a window has given pages of these positions back")
+        at = torch.arange(first, first + count, dtype=torch.int32, device=self.device)
+        if spec.eight_bit:
+            from ..ops import native
+
+            out = [torch.empty((count, spec.num_kv_heads, spec.head_dim), dtype=dtype or self.dtype, device=self.device) for _ in range(2)]
+            status = torch.zeros(1, dtype=torch.int32, device=self.device)
+            pages = torch.tensor([table.pages], dtype=torch.int32, device=self.device)
+            native.kv8_read(k_cache, v_cache, *self.scales_of_run(run), pages, at, torch.zeros_like(at), *out, status)
+            return tuple(out)
+        page = torch.tensor(places, dtype=torch.long, device=self.device)
+        slot = at.long() % self.page_size
+        return tuple(c[page, :, slot].to(dtype or c.dtype) for c in (k_cache, v_cache))
+
     def view(self, run: int):
         """The CacheView a mixer gets for run ``run``."""
         from ..parts.base import CacheView
@@ -255,6 +308,7 @@ class CacheManager:
         kv = self.kv_of_run(run) if run in self._run_group and self.groups[self._run_group[run][0]].storage is not None else None
         return CacheView(
             kv=kv,
+            scales=None if kv is None else self.scales_of_run(run),
             group=self.group_of_run(run),
             owns=run not in self.shares,
             state=self.state_of_run(run),

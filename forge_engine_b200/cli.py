@@ -37,6 +37,8 @@ def build_parser() -> argparse.ArgumentParser:
     generate.add_argument("--prompt-ids", action="append", required=True,
                           help="comma-separated token ids; may be given more than once")
     generate.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16")
+    generate.add_argument("--cache-dtype", choices=("auto", "float8"), default="auto",
+                          help="float8: keys and values in 8 bits (bfloat16 engine, plain attention layers)")
     generate.add_argument("--device", default="cuda:0")
     generate.add_argument("--max-new-tokens", type=int, default=256)
     generate.add_argument("--temperature", type=float, default=0.0)
@@ -109,6 +111,7 @@ def run_generate(args: argparse.Namespace) -> int:
         min_p=args.min_p,
         seed=args.seed,
         dtype=args.dtype,
+        cache_dtype=None if args.cache_dtype == "auto" else args.cache_dtype,
     )
     scheduler_config = SchedulerConfig(
         max_requests=args.max_requests,

@@ -23,11 +23,16 @@ class EngineConfig:
     min_p: float = 0.0
     seed: int | None = None
     dtype: str = "bfloat16"
+    cache_dtype: str | None = None     # "float8": keys and values in 8 bits; None: in ``dtype``
 
     def __post_init__(self) -> None:
         self.sampling_params()
         if self.dtype not in ("bfloat16", "float32"):
             raise ValueError("dtype must be 'bfloat16' or 'float32'")
+        if self.cache_dtype not in (None, "float8"):
+            raise ValueError("cache_dtype must be None or 'float8'")
+        if self.cache_dtype == "float8" and self.dtype != "bfloat16":
+            raise ValueError("an 8-bit cache goes with dtype 'bfloat16'")
 
     def sampling_params(self) -> SamplingParams:
         return SamplingParams(

@@ -161,11 +161,16 @@ __device__ __forceinline__ void value_stretch(const unsigned char* vs, int k0, c
     const unsigned lo0 = __byte_perm(w[0][c], w[1][c], 0x5140), lo1 = __byte_perm(w[0][c], w[1][c], 0x7362);
     const unsigned hi0 = __byte_perm(w[2][c], w[3][c], 0x5140), hi1 = __byte_perm(w[2][c], w[3][c], 0x7362);
     constexpr int N0 = BASE / 8;
-    mma_f16(o[N0 + 4 * c], a, kv8_half2((unsigned short)lo0), kv8_half2((unsigned short)hi0));
-    mma_f16(o[N0 + 4 * c + 1], a, kv8_half2((unsigned short)(lo0 >> 16)), kv8_half2((unsigned short)(hi0 >> 16)));
+    unsigned b0[4], b1[4];
+    kv8_halves(lo0, b0[0], b0[1]);
+    kv8_halves(hi0, b1[0], b1[1]);
+    mma_f16(o[N0 + 4 * c], a, b0[0], b1[0]);
+    mma_f16(o[N0 + 4 * c + 1], a, b0[1], b1[1]);
     if constexpr (W > 2) {
-      mma_f16(o[N0 + 4 * c + 2], a, kv8_half2((unsigned short)lo1), kv8_half2((unsigned short)hi1));
-      mma_f16(o[N0 + 4 * c + 3], a, kv8_half2((unsigned short)(lo1 >> 16)), kv8_half2((unsigned short)(hi1 >> 16)));
+      kv8_halves(lo1, b0[2], b0[3]);
+      kv8_halves(hi1, b1[2], b1[3]);
+      mma_f16(o[N0 + 4 * c + 2], a, b0[2], b1[2]);
+      mma_f16(o[N0 + 4 * c + 3], a, b0[3], b1[3]);
     }
   }
 }
@@ -203,8 +208,11 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
     }
     if constexpr ((D & 16) != 0) w[D / 16 - 1] = *reinterpret_cast<const unsigned*>(stage + row * D + D - 16 + 4 * t);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-      mma_f16(c[n], q.a[i], kv8_half2((unsigned short)w[i]), kv8_half2((unsigned short)(w[i] >> 16)));
+    for (int i = 0; i < D / 16; ++i) {
+      unsigned b0, b1;
+      kv8_halves(w[i], b0, b1);
+      mma_f16(c[n], q.a[i], b0, b1);
+    }
     // keys 8 n + 2 t and the next one
     const float2 up = *reinterpret_cast<const float2*>(of_key + 8 * n + 2 * t);
     const float2 add = *reinterpret_cast<const float2*>(of_key + STEP + 8 * n + 2 * t);
@@ -267,20 +275,23 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
 // A warp goes its own way: it copies its keys into a ring of its own, a step ahead, and waits for nobody (with a ring of the
 // block and a barrier a tile, 64 keys of one head took 1.7 us a block whatever else ran).  A lane looks after one key: its
 // page, two steps ahead, its place and its scales.
-// grid: (spans x row tiles, entries, kv heads); a block takes `span` key tiles of its unit.
+// grid: (spans, row tiles - single tokens: entries -, kv heads); a block takes `span` key tiles of its unit.
 template <bool PORTION>
 __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
   pdl_trigger();
   pdl_wait();
-  const int entry = blockIdx.y, kvh = blockIdx.z;
-  const int unit = blockIdx.x / p.spans, piece = blockIdx.x - unit * p.spans;
+  const int slot = blockIdx.y, kvh = blockIdx.z, piece = blockIdx.x;
+  int entry = slot, unit = 0;
+  if constexpr (PORTION) {
+    const Slot<UNIT> at(p, slot);
+    entry = at.entry;
+    unit = at.unit;
+  }
   const Entry e(p, entry);
-  const int rows = e.n_new * p.groups;
-  if (rows <= p.row_lo || rows > p.row_hi) return;
-  const int row0 = unit * UNIT;
-  if (row0 >= rows) return;
+  const int rows = e.n_new * p.groups, row0 = unit * UNIT;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
   const int rows_end = min(rows, row0 + UNIT);
   const Walk<KEYS> walk(p, e.start, row0, rows_end);
   const int pieces = pieces_of(p, walk.count);
@@ -356,7 +367,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 2);
   }
-  float* ws = p.ws + ((((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans + piece) * UNIT * (D + 2);
+  float* ws = p.ws + (((size_t)slot * p.nkv + kvh) * p.spans + piece) * UNIT * (D + 2);
   if constexpr (PORTION) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -431,49 +442,48 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
 }
 
 template <bool PORTION>
-int launch_mma(Kv8Attention p, int entries, int max_new, cudaStream_t stream) {
+int launch_mma(Kv8Attention p, cudaStream_t stream) {
   constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
-  const long long max_rows = (long long)max_new * p.groups;
-  p.units = PORTION ? (int)((max_rows + UNIT - 1) / UNIT) : 1;
-  if ((long long)p.units * p.spans > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
+  const long long slots = PORTION ? portion_slots(p.entries, p.total_tokens, p.groups, UNIT) : p.entries;
+  if (slots > 65535) return FE_ERR_TOO_LARGE;
+  p.slots = (int)slots;
   const cudaError_t err = cudaFuncSetAttribute(attn_kv8_mma_kernel<PORTION>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM);
   if (err != cudaSuccess) return (int)err;
-  int rc = fe_launch_dependent(attn_kv8_mma_kernel<PORTION>, dim3((unsigned)(p.units * p.spans), (unsigned)entries, (unsigned)p.nkv),
-                               dim3(THREADS), MMA_SMEM, stream, p);
+  int rc = fe_launch_dependent(attn_kv8_mma_kernel<PORTION>, dim3((unsigned)p.spans, (unsigned)p.slots, (unsigned)p.nkv), dim3(THREADS), MMA_SMEM,
+                               stream, p);
   if (rc == 0 && p.spans > 1)
-    rc = fe_launch_dependent(attn_kv8_join_kernel<UNIT, KEYS>, dim3((unsigned)(p.units * (UNIT / JOIN_WARPS)), (unsigned)entries, (unsigned)p.nkv),
-                             dim3(32 * JOIN_WARPS), 0, stream, p);
+    rc = launch_join<UNIT, KEYS, PORTION>(p, stream);
   return rc;
 }
 
 }  // namespace
 
-// 32-bit numbers of workspace that `entries` of up to `max_new` tokens need, cut into `spans` pieces.
-FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, int nkv, int groups, int max_new, int spans) {
+// 32-bit numbers of workspace that `entries` of `total_tokens` tokens in all need, cut into `spans` pieces.
+FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, int nkv, int groups, int total_tokens, int spans) {
   if (spans <= 1) return 0;
 #if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
-  const long long unit = portion ? PORTION_UNIT : ROWS;
+  const int unit = portion ? PORTION_UNIT : ROWS;
 #else
-  const long long unit = portion ? ROWS * WARPS : ROWS;
+  const int unit = portion ? ROWS * WARPS : ROWS;
 #endif
-  const long long units = portion ? ((long long)max_new * groups + unit - 1) / unit : 1;
-  return (long long)entries * nkv * units * spans * unit * (D + 2);
+  const long long slots = portion ? portion_slots(entries, total_tokens, groups, unit) : entries;
+  return slots * nkv * spans * unit * (D + 2);
 }
 
 // The entries of a step with at most 16 rows (new tokens x heads per kv head) if single_spans is above zero, the others
 // if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
-                                      int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new,
-                                      int total_tokens, int window, int keep_first, float scale, int single_span,
+                                      int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int total_tokens,
+                                      int window, int keep_first, float scale, int single_span,
                                       int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
                                       cudaStream_t stream) {
-  if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
+  if (entries <= 0 || total_tokens <= 0) return 0;
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
   if (single_spans < 0 || portion_spans < 0 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
   if ((single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
   if ((long long)num_pages * nkv > 0x7fffffffLL / page_size) return FE_ERR_TOO_LARGE;       // rows of a cache: 31 bits
-  if (entries > 65535 || nkv > 65535 || (long long)max_new * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
+  if (entries > 65535 || nkv > 65535 || (long long)total_tokens * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
   if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) ||
       q_stride % 4)
     return FE_ERR_BAD_ALIGN;
@@ -485,19 +495,20 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   for (int s = 0; s < 31; ++s)
     if (page_size == 1 << s) p.page_shift = s;
   p.nkv = nkv; p.groups = groups; p.cu_tokens = cu_tokens; p.starts = starts; p.total_tokens = total_tokens;
+  p.entries = entries; p.slots = 0;
   p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.ws = workspace;
   if (single_spans > 0) {
     p.row_lo = 0; p.row_hi = ROWS; p.span = single_span; p.spans = single_spans;
-    const int rc = launch_mma<false>(p, entries, max_new, stream);
+    const int rc = launch_mma<false>(p, stream);
     if (rc) return rc;
   }
   if (portion_spans > 0) {
     p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans;
 #if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
-    const int rc = launch_portion(p, entries, max_new, stream);
+    const int rc = launch_portion(p, stream);
 #else
-    const int rc = launch_mma<true>(p, entries, max_new, stream);
+    const int rc = launch_mma<true>(p, stream);
 #endif
     if (rc) return rc;
   }

@@ -27,8 +27,9 @@ struct Kv8Attention {
   int* status;
   int row_lo, row_hi;      // entries with row_lo < rows <= row_hi
   int span, spans;         // a block takes `span` key tiles of a unit; the grid holds `spans` of them
-  int units;               // row tiles of the longest entry
-  float* ws;               // [entries, nkv, units, spans][rows of a unit x (D + 2)]: see piece_element
+  int entries;
+  int slots;               // row tiles of all entries, at most: see Slot
+  float* ws;               // [slots, nkv, spans][rows of a unit x (D + 2)]: see piece_element
 };
 
 // The key tiles (of TILE keys) that the rows [row0, row0 + n) of an entry see: first the tiles that hold kept
@@ -71,6 +72,26 @@ __device__ __forceinline__ int key_page(const Kv8Attention& p, const int* table,
   return key < key_end && logical < p.max_pages ? __ldg(table + logical) : -1;
 }
 
+// Which row tile of which entry a block takes.  Entry e's tiles of UNIT rows are slots floor(cu[e] G / UNIT) + e on: they
+// never meet the next entry's, and there are no more slots than total tokens * G / UNIT + entries.  A warp finds the
+// entry, 32 of them at a time.
+template <int UNIT> struct Slot {
+  int entry, unit;
+  __device__ __forceinline__ Slot(const Kv8Attention& p, int slot) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int e0 = 0; e0 < p.entries; e0 += 32) {
+      const int e = e0 + lane;
+      const bool is = e < p.entries && (int)((long long)p.cu_tokens[e] * p.groups / UNIT) + e <= slot;
+      const unsigned votes = __ballot_sync(0xffffffffu, is);
+      before += __popc(votes);
+      if (votes != 0xffffffffu) break;
+    }
+    entry = max(before - 1, 0);
+    unit = slot - ((int)((long long)p.cu_tokens[entry] * p.groups / UNIT) + entry);
+  }
+};
+
 // Row (page, head, slot) of a key in its page; a page that is not there gives row 0 and false.
 __device__ __forceinline__ bool key_row(const Kv8Attention& p, int page, int kvh, int key, long long* row) {
   const bool there = page >= 0 && page < p.num_pages;
@@ -101,30 +122,45 @@ template <int UNIT> __device__ __forceinline__ size_t piece_element(int r, int d
   return ((size_t)(d >> 3) * UNIT + r) * 8 + (d & 7);
 }
 
-constexpr int JOIN_WARPS = 4;
+// Row tiles of UNIT rows of a call's portions, at most.
+inline long long portion_slots(int entries, int total_tokens, int groups, int unit) {
+  return (long long)total_tokens * groups / unit + entries;
+}
 
-// Joins the pieces of a unit's rows, in the order of the keys: a warp a row, a lane D / 32 (at least two)
-// neighbouring columns; the lanes work out 32 pieces' shares at a time.
-// grid: (units x UNIT / 4, entries, kv heads)
-template <int UNIT, int TILE>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Attention p) {
+// Joins the pieces of a unit's rows, in the order of the keys: a lane takes D / 32 (at least two) neighbouring columns
+// of a row and works out one piece's share of 32.  Portions have few pieces and many rows: four rows a block, a warp
+// each.  A single token's row may have a hundred pieces: a block a row, its eight warps every eighth piece, their sums
+// joined in the order of the warps (one warp a row: 13.8 us for 103 pieces).
+// grid: (rows of the slots / rows of a block, kv heads)
+template <bool PORTION> constexpr int JOIN_ROWS = PORTION ? 4 : 1;
+template <bool PORTION> constexpr int JOIN_WARPS = PORTION ? 4 : 8;
+
+template <int UNIT, int TILE, bool PORTION>
+__global__ void __launch_bounds__(32 * JOIN_WARPS<PORTION>) attn_kv8_join_kernel(Kv8Attention p) {
   constexpr int COLUMNS = D >= 128 ? 4 : 2, LANES_D = 32 * COLUMNS;
   constexpr int PASSES = (D + LANES_D - 1) / LANES_D;
+  constexpr int BLOCKS = UNIT / JOIN_ROWS<PORTION>, SHARE = PORTION ? 1 : JOIN_WARPS<PORTION>;
+  __shared__ float sums[SHARE][PASSES * LANES_D], dens[SHARE];
   pdl_trigger();
   pdl_wait();
-  constexpr int BLOCKS = UNIT / JOIN_WARPS;
-  const int unit = blockIdx.x / BLOCKS, entry = blockIdx.y, kvh = blockIdx.z, lane = threadIdx.x & 31;
+  const int slot = blockIdx.x / BLOCKS, kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int entry = slot, unit = 0;
+  if constexpr (PORTION) {
+    const Slot<UNIT> at(p, slot);
+    entry = at.entry;
+    unit = at.unit;
+  }
   const Entry e(p, entry);
   const int rows = e.n_new * p.groups, row0 = unit * UNIT;
-  if (rows <= p.row_lo || rows > p.row_hi || row0 >= rows) return;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
   const int rows_end = min(rows, row0 + UNIT);
-  const int r = (blockIdx.x - unit * BLOCKS) * JOIN_WARPS + (threadIdx.x >> 5);
+  const int r = (blockIdx.x - slot * BLOCKS) * JOIN_ROWS<PORTION> + (PORTION ? warp : 0);
   if (row0 + r >= rows_end) return;
   const Walk<TILE> walk(p, e.start, row0, rows_end);
   const int pieces = pieces_of(p, walk.count);
   if (pieces == 1) return;
   const size_t step = (size_t)UNIT * (D + 2);
-  const float* ws = p.ws + (((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans * step;
+  const float* ws = p.ws + ((size_t)slot * p.nkv + kvh) * p.spans * step;
   const float* ml = ws + (size_t)UNIT * D + 2 * r;
   float big = -INFINITY;
   for (int s = lane; s < pieces; s += 32) big = fmaxf(big, ml[s * step]);
@@ -134,18 +170,19 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
   for (int i = 0; i < PASSES; ++i)
 #pragma unroll
     for (int c = 0; c < COLUMNS; ++c) num[i][c] = 0.f;
-  for (int s0 = 0; s0 < pieces; s0 += 32) {
-    float mine = 0.f;
-    if (s0 + lane < pieces) {
-      const float m = ml[(s0 + lane) * step], l = ml[(s0 + lane) * step + 1];
-      mine = piece_share(m, l, big);
-      den += l * mine;
+  const int first = PORTION ? 0 : warp, mine = (pieces - first + SHARE - 1) / SHARE;        // pieces first, first + SHARE, ...
+  for (int k0 = 0; k0 < mine; k0 += 32) {
+    float share = 0.f;
+    if (k0 + lane < mine) {
+      const float* at = ml + (size_t)(first + (k0 + lane) * SHARE) * step;
+      share = piece_share(at[0], at[1], big);
+      den += at[1] * share;
     }
-    const int here = min(32, pieces - s0);
-#pragma unroll 4
-    for (int s = 0; s < here; ++s) {
-      const float f = __shfl_sync(0xffffffffu, mine, s);
-      const float* src = ws + (s0 + s) * step;
+    const int here = min(32, mine - k0);
+#pragma unroll 8
+    for (int k = 0; k < here; ++k) {
+      const float f = __shfl_sync(0xffffffffu, share, k);
+      const float* src = ws + (size_t)(first + (k0 + k) * SHARE) * step;
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int d = i * LANES_D + lane * COLUMNS;
@@ -161,19 +198,43 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
     }
   }
   den = warp_sum(den);
+  if constexpr (!PORTION) {
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int d = i * LANES_D + lane * COLUMNS;
-    if (D % LANES_D == 0 || d < D) {
+    for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-      for (int c = 0; c < COLUMNS; ++c) store_row(p, e, kvh, row0 + r, d + c, den == 0.f ? 0.f : num[i][c] / den);
+      for (int c = 0; c < COLUMNS; ++c) sums[warp][i * LANES_D + lane * COLUMNS + c] = num[i][c];
+    if (lane == 0) dens[warp] = den;
+    __syncthreads();
+    den = 0.f;
+#pragma unroll
+    for (int w = 0; w < SHARE; ++w) den += dens[w];
+    for (int d = threadIdx.x; d < D; d += 32 * SHARE) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < SHARE; ++w) x += sums[w][d];
+      store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : x / den);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int d = i * LANES_D + lane * COLUMNS;
+      if (D % LANES_D == 0 || d < D) {
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) store_row(p, e, kvh, row0 + r, d + c, den == 0.f ? 0.f : num[i][c] / den);
+      }
     }
   }
 }
 
+template <int UNIT, int TILE, bool PORTION>
+inline int launch_join(const Kv8Attention& p, cudaStream_t stream) {
+  return fe_launch_dependent(attn_kv8_join_kernel<UNIT, TILE, PORTION>, dim3((unsigned)(p.slots * (UNIT / JOIN_ROWS<PORTION>)), (unsigned)p.nkv),
+                             dim3(32 * JOIN_WARPS<PORTION>), 0, stream, p);
+}
+
 #if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
 constexpr int PORTION_UNIT = 256, PORTION_TILE = 128;      // rows of a block and keys of a tile of the tcgen05 kernel
-int launch_portion(Kv8Attention p, int entries, int max_new, cudaStream_t stream);
+int launch_portion(Kv8Attention p, cudaStream_t stream);
 #endif
 
 }  // namespace kv8

@@ -194,15 +194,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
 
   pdl_trigger();
   pdl_wait();
-  const int kvh = blockIdx.x, entry = blockIdx.y;
   // blocks start in the order of x, y, z: the row tiles that see most keys first
-  const int z = gridDim.z - 1 - blockIdx.z;
-  const int unit = z / p.spans, piece = z - unit * p.spans;
-  const Entry e(p, entry);
-  const int rows = e.n_new * p.groups;
-  if (rows <= p.row_lo || rows > p.row_hi) return;
-  const int row0 = unit * PORTION_UNIT;
-  if (row0 >= rows) return;
+  const int kvh = blockIdx.x, slot = gridDim.y - 1 - blockIdx.y, piece = blockIdx.z;
+  const Slot<PORTION_UNIT> at(p, slot);
+  const Entry e(p, at.entry);
+  const int rows = e.n_new * p.groups, row0 = at.unit * PORTION_UNIT;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
   const Walk<KEYS> walk(p, e.start, row0, min(rows, row0 + PORTION_UNIT));
   const int pieces = pieces_of(p, walk.count);
   if (piece >= pieces) return;
@@ -237,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
 
   if (warp >= SOFTMAX_WARPS && warp < MMA_WARP) {
     // ---- staging ----
-    const int* table = p.block_table + (size_t)entry * p.max_pages;
+    const int* table = p.block_table + (size_t)at.entry * p.max_pages;
     // Piece j of this lane is 16 bytes of one of the warp's rows, unit w + 8 j; the lanes of a unit lie so that eight
     // neighbours store their 32 bytes of bfloat16 without meeting in a bank.  A lane looks after one of the warp's
     // rows - its page, its place and its scales - and the others ask it.
@@ -305,8 +302,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
         unsigned x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          x[2 * k] = bf16_of_half(kv8_half2((unsigned short)words[k]), up);
-          x[2 * k + 1] = bf16_of_half(kv8_half2((unsigned short)(words[k] >> 16)), up);
+          unsigned lo, hi;
+          kv8_halves(words[k], lo, hi);
+          x[2 * k] = bf16_of_half(lo, up);
+          x[2 * k + 1] = bf16_of_half(hi, up);
         }
         if (large) {
           const __nv_bfloat162 more = __float2bfloat162_rn(__int_as_float((127 + max(ex - 15, 0)) << 23));
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
     if (ok) {
       const int ur = x * TILE_ROWS + r;
       const float by = pieces > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* ws = p.ws + ((((size_t)entry * p.nkv + kvh) * p.units + unit) * p.spans + piece) * (size_t)PORTION_UNIT * (D + 2);
+      float* ws = p.ws + (((size_t)slot * p.nkv + kvh) * p.spans + piece) * (size_t)PORTION_UNIT * (D + 2);
       // a finished warp's 32 rows pass through its queries' place, so that whole rows go out
       unsigned char* rows_here = q_tiles + x * 2 * CODE_TILE + quarter * 32 * D * 2;
 #pragma unroll 1
@@ -665,16 +664,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
 
 namespace kv8 {
 
-int launch_portion(Kv8Attention p, int entries, int max_new, cudaStream_t stream) {
-  p.units = (int)(((long long)max_new * p.groups + PORTION_UNIT - 1) / PORTION_UNIT);
-  if ((long long)p.units * p.spans > 65535) return FE_ERR_TOO_LARGE;
+int launch_portion(Kv8Attention p, cudaStream_t stream) {
+  const long long slots = portion_slots(p.entries, p.total_tokens, p.groups, PORTION_UNIT);
+  if (slots > 65535 || p.spans > 65535) return FE_ERR_TOO_LARGE;
+  p.slots = (int)slots;
   const cudaError_t err = cudaFuncSetAttribute(attn_kv8_portion_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
   if (err != cudaSuccess) return (int)err;
-  int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)entries, (unsigned)(p.units * p.spans)), dim3(THREADS),
-                               SMEM, stream, p);
+  int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)p.slots, (unsigned)p.spans), dim3(THREADS), SMEM, stream, p);
   if (rc == 0 && p.spans > 1)
-    rc = fe_launch_dependent(attn_kv8_join_kernel<PORTION_UNIT, PORTION_TILE>, dim3((unsigned)(p.units * (PORTION_UNIT / JOIN_WARPS)), (unsigned)entries, (unsigned)p.nkv),
-                             dim3(32 * JOIN_WARPS), 0, stream, p);
+    rc = launch_join<PORTION_UNIT, PORTION_TILE, true>(p, stream);
   return rc;
 }
 

@@ -53,3 +53,9 @@ __device__ __forceinline__ unsigned kv8_half2(unsigned short codes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(codes));
   return r;
 }
+
+// four codes as two pairs of half-precision numbers
+__device__ __forceinline__ void kv8_halves(unsigned codes, unsigned& lo, unsigned& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}

@@ -58,6 +58,7 @@ class Engine:
             page_size=scheduler_config.block_size,
             num_pages=scheduler_config.block_capacity,
             max_requests=scheduler_config.max_requests,
+            cache_dtype=engine_config.cache_dtype,
         )
         return cls(runner, engine_config, scheduler_config)
 
@@ -81,6 +82,7 @@ class Engine:
             page_size=scheduler_config.block_size,
             num_pages=scheduler_config.block_capacity,
             max_requests=scheduler_config.max_requests,
+            cache_dtype=engine_config.cache_dtype,
         )
         return cls(runner, engine_config, scheduler_config)
 

@@ -13,7 +13,7 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..config.registry import read_model_config
-from ..errors import ForgeEngineError, KVCacheCapacityError
+from ..errors import ConfigError, ForgeEngineError, KVCacheCapacityError
 from ..models.decoder import DecoderModel
 from ..ops import native
 from ..parts.base import BuildContext
@@ -25,6 +25,22 @@ from .timing import StepTimer
 
 DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32, "bf16": torch.bfloat16,
           "fp32": torch.float32}
+
+
+CACHE_DTYPES = (None, "float8")
+
+
+def check_cache(needs: list, cache_dtype: str | None) -> None:
+    """Refuse a model some of whose layers cannot keep what an 8-bit cache asks of all layers with paged keys."""
+    if cache_dtype is None:
+        return
+    paged = [(run, need.kv) for run, need in enumerate(needs) if need is not None and need.kv is not None]
+    if not paged:
+        raise ConfigError("cache_dtype='float8': the model keeps no keys and values")
+    for run, kv in paged:
+        if not kv.eight_bit:
+            raise ConfigError(f"cache_dtype='float8': the layer of run {run} has no form over an 8-bit cache (plain grouped-query "
+                              "attention of the bfloat16 engine has one, with a window and a rotation of whole multiples of 8)")
 
 
 def resolve_dtype(name) -> torch.dtype:
@@ -52,6 +68,7 @@ class ModelRunner:
             self.timer = self.ctx.timer = StepTimer()
             use_graphs = False
         needs, shares = model.cache_needs()
+        check_cache(needs, self.ctx.cache_dtype)
         self.cache = CacheManager(
             needs,
             page_size=page_size,
@@ -70,8 +87,9 @@ class ModelRunner:
     @classmethod
     def from_folder(cls, folder: str | Path, *, dtype="bfloat16", device="cuda:0", page_size: int = 16,
                     num_pages: int = 1024, max_requests: int = 16, use_graphs: bool = True,
-                    timing: bool = False) -> "ModelRunner":
-        """Model class by config.json's architecture, weights by tensor name."""
+                    timing: bool = False, cache_dtype: str | None = None) -> "ModelRunner":
+        """Model class by config.json's architecture, weights by tensor name.  ``cache_dtype`` "float8" keeps keys
+        and values in 8 bits (half a bfloat16 cache's bytes); None in the engine's dtype."""
         native.require_cuda()
         native.lib()
         engine_dtype = resolve_dtype(dtype)
@@ -83,12 +101,12 @@ class ModelRunner:
         weights = open_checkpoint(folder, expected, engine_dtype, device, optional)
         return cls.from_tensors(spec, weights, dtype=engine_dtype, device=device, page_size=page_size,
                                 num_pages=num_pages, max_requests=max_requests, use_graphs=use_graphs,
-                                architecture=arch, timing=timing)
+                                architecture=arch, timing=timing, cache_dtype=cache_dtype)
 
     @classmethod
     def from_random(cls, config: dict, seed: int, *, dtype="bfloat16", device="cuda:0", page_size: int = 16,
                     num_pages: int = 1024, max_requests: int = 16, std: float = 0.02,
-                    use_graphs: bool = True, timing: bool = False) -> "ModelRunner":
+                    use_graphs: bool = True, timing: bool = False, cache_dtype: str | None = None) -> "ModelRunner":
         """Random weights drawn on the device (benchmark-sized models never touch the disk)."""
         native.require_cuda()
         native.lib()
@@ -97,18 +115,20 @@ class ModelRunner:
         weights = RandomTensors(arch.expected_tensors(spec), seed, std=std, dtype=engine_dtype, device=device)
         return cls.from_tensors(spec, weights, dtype=engine_dtype, device=device, page_size=page_size,
                                 num_pages=num_pages, max_requests=max_requests, use_graphs=use_graphs,
-                                architecture=arch, timing=timing)
+                                architecture=arch, timing=timing, cache_dtype=cache_dtype)
 
     @classmethod
     def from_tensors(cls, spec, weights: dict, *, dtype, device, page_size: int, num_pages: int,
                      max_requests: int, use_graphs: bool = True, architecture=None,
-                     timing: bool = False) -> "ModelRunner":
+                     timing: bool = False, cache_dtype: str | None = None) -> "ModelRunner":
         """``architecture`` (a registry entry) assembles the model; None builds the decoder of
         ``models/decoder.py``."""
         native.require_cuda()
         native.lib()
         status = torch.zeros(1, dtype=torch.int32, device=device)
-        ctx = BuildContext(dtype=resolve_dtype(dtype), device=torch.device(device), status=status)
+        if cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype={cache_dtype!r}; known: 'float8', or None for the engine's dtype")
+        ctx = BuildContext(dtype=resolve_dtype(dtype), device=torch.device(device), status=status, cache_dtype=cache_dtype)
         with torch.cuda.device(ctx.device):
             try:
                 model = DecoderModel(spec, weights, ctx) if architecture is None else architecture.build(spec, weights, ctx)

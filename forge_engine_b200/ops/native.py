@@ -1913,7 +1913,7 @@ def kv8_lib(head_dim: int):
             raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
         p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
         fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
-        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, p, p, p]
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, f, i, i, i, i, p, p, p]
         fn.restype = c_int
         size.argtypes = [i, i, i, i, i, i]
         size.restype = ll
@@ -2108,12 +2108,14 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out, rows=(q,))
     single_span, single_spans, portion_span, portion_spans = plan
     groups = num_q_heads // nkv
+    if max_new * groups <= KV8_SINGLE_ROWS:
+        portion_spans = 0
     fn, size = kv8_lib(d)
     with torch.cuda.device(q.device):
         # the pieces of a cut entry meet in a buffer of the call's own: calls on other streams, and captured ones, have theirs
-        numbers = max(size(0, n_entries, nkv, groups, max_new, single_spans), size(1, n_entries, nkv, groups, max_new, portion_spans))
+        numbers = max(size(0, n_entries, nkv, groups, n, single_spans), size(1, n_entries, nkv, groups, n, portion_spans))
         workspace = torch.empty(numbers, dtype=torch.float32, device=q.device) if numbers else None
         check(fn(ptr(q), q_stride, ptr(out), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table),
-                 block_table.shape[1], page_size, num_pages, nkv, groups, ptr(cu_tokens), ptr(starts), n_entries, max_new, n, window,
+                 block_table.shape[1], page_size, num_pages, nkv, groups, ptr(cu_tokens), ptr(starts), n_entries, n, window,
                  keep_first, float(scale), single_span, single_spans, portion_span, portion_spans, ptr(workspace), ptr(status),
                  stream()), "attention_kv8")

@@ -124,6 +124,8 @@ def _choose_splits(tile_counts: tuple, kv_heads: int, balanced: bool, DECODE_SLO
 
 
 class GQAttention(Mixer):
+    eight_bit = False     # keeps its keys and values in 8 bits
+
     @property
     def graph_safe(self) -> bool:
         """The kernels here are; a position encoding that rewrites q and k itself decides."""
@@ -239,9 +241,14 @@ class GQAttention(Mixer):
                            and self.chunk is None and self.keep_first == 0 and self.softcap is None and self.query_temperature is None
                            and self.slopes is None and self.distance_bias is None and self.sinks is None
                            and not self.head_gate and not self.output_gate)
+        # keys and values in 8 bits: a plain layer of the bfloat16 engine, rotated (if at all) by a table of angles
+        rotary = self.position.rotary()
+        self.eight_bit = (ctx.cache_dtype == "float8" and not self.general and ctx.dtype == torch.bfloat16 and native.kv8_takes(self.d)
+                          and (rotary is None or (hasattr(self.position, "table") and rotary[1] % 8 == 0)))
         self._slots = None
         self.plan_key = ("gqa_attention", self.nq, self.nkv, self.d, spec.window) + (
-            ("general", self.dv, self.parts, self.keep_first, self.chunk) if self.general and not self.plain_core else ())
+            ("general", self.dv, self.parts, self.keep_first, self.chunk) if self.general and not self.plain_core else ()) + (
+            ("float8",) if self.eight_bit else ())
         self.last_splits = None   # what the last step's decode entries ran with (0: balanced kernel)
 
     @staticmethod
@@ -311,7 +318,7 @@ class GQAttention(Mixer):
     def cache_needs(self) -> CacheNeeds:
         key = self.parts * self.d          # a differential layer caches both keys of a head in one row
         return CacheNeeds(kv=PagedKVSpec(self.nkv, key, self.spec.window, None if self.dv == key else self.dv,
-                                         self.keep_first, getattr(self.spec, "chunk", None)))
+                                         self.keep_first, getattr(self.spec, "chunk", None), self.eight_bit))
 
     def decode_slots(self) -> int:
         """Blocks of the decode kernels this device holds at once: what the balanced kernel
@@ -341,6 +348,8 @@ class GQAttention(Mixer):
         (a block that fuses ``o_proj`` with what follows takes them from here)."""
         if self.general:
             return self._attend_general(x, batch, cache)
+        if cache.scales is not None:
+            return self._attend_eight_bit(x, batch, cache)
         with self.ctx.section("mixer.qkv_rope_cache"):
             qkv = self._project(x, batch, cache)
         k_cache, v_cache = cache.kv
@@ -356,6 +365,31 @@ class GQAttention(Mixer):
                     self.spec.window, self.spec.scale, out, self.nq, self.ctx.status,
                     entries=(batch.cu_tokens, batch.n_entries, batch.max_new),
                 )
+        return out
+
+    def _attend_eight_bit(self, x, batch, cache: CacheView):
+        """The plain layer over an 8-bit cache: one kernel norms and rotates q and k and quantises k and v into their
+        pages, and the attention reads the codes.  Up to 64 tokens the projection leaves 32-bit sums."""
+        caches = (*cache.kv, *cache.scales)
+        table = batch.group_tables[cache.group]
+        q_end, k_end = self.nq * self.d, (self.nq + self.nkv) * self.d
+        with self.ctx.section("mixer.qkv_rope_cache"):
+            qkv = self.qkv_proj(x, out_dtype=torch.float32 if self.qkv_proj._tc5_ok(x) else None)
+            rotary, angles = self.position.rotary(), None
+            if rotary is None:
+                self.position.apply(qkv, self.nq, self.nkv, self.d, batch)
+            elif rotary[1]:
+                angles = self.position.table(batch)
+            q = torch.empty((x.shape[0], q_end), dtype=torch.bfloat16, device=x.device)
+            native.kv8_write(qkv[:, q_end:k_end] if cache.owns else None, qkv[:, k_end:] if cache.owns else None,
+                             batch.positions, batch.token_entry, *caches, table, self.ctx.status, q=qkv[:, :q_end], q_out=q,
+                             q_norm=self.q_norm, k_norm=self.k_norm, eps=self.spec.qk_norm_eps, table=angles)
+        if self.plan_key not in batch.plans:
+            self.plan_step(batch.entries, caches[0].shape[2], batch.plans)
+        out = torch.empty_like(q)
+        with self.ctx.section("mixer.attention"):
+            native.attention_kv8(q, *caches, table, batch.cu_tokens, batch.starts, batch.n_entries, batch.max_new, self.nq,
+                                 self.spec.window, 0, self.spec.scale, out, self.ctx.status, batch.plans[self.plan_key])
         return out
 
     def _attend_general(self, x, batch, cache: CacheView):
@@ -520,6 +554,11 @@ class GQAttention(Mixer):
         rest the prefill kernel; both may run in one step.  (run prefill, run decode, splits
         of the decode kernel - 0: the kernel that spreads all tiles evenly) under this
         mixer's key; layers with the same geometry share it."""
+        if self.eight_bit:
+            if self.plan_key not in plans:
+                plans[self.plan_key] = native.kv8_plan([(start, count) for _, start, count in entries], self.nq, self.nkv, self.d,
+                                                       self.spec.window)
+            return
         if self.general and not self.plain_core:
             # the general kernels: (how many blocks share a row tile's keys, whether entries go
             # to the tcgen05 prefill kernel, whether entries go to the general kernel)

@@ -42,6 +42,7 @@ class BuildContext:
     dtype: object  # torch.float32 or torch.bfloat16: dtype of activations and of the KV cache
     device: object
     status: object  # int32[1] device word kernels set error bits in
+    cache_dtype: str | None = None  # "float8": layers that can keep their keys and values in 8 bits do
     timer: object = None  # None, or an object whose ``section(name)`` brackets a part's call with events
 
     def section(self, name: str):
@@ -75,6 +76,8 @@ class CacheView:
     owns: bool
     state: object = None
     own_state: object = None
+    # (scales of the keys, of the values) [pages, kv_heads, page_size] where ``kv`` is an 8-bit cache
+    scales: tuple | None = None
     # further states of the run by name (``CacheNeeds.states``), each [max_requests + 1, *shape]
     states: dict = field(default_factory=dict)
 
