@@ -8,7 +8,7 @@
 //   b = the largest |x| of a head's vector (a maximum over a group of lanes, on the bits of |x|, so that
 //       infinities and NaN win),  e = least with b <= 448 * 2^e,  codes = round(x * 2^-e)
 // k and v are quantised from the unrounded 32-bit values: one rounding between the projection and the page.
-#include <cuda_fp16.h>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -38,11 +38,20 @@ __device__ __forceinline__ long long kv8_row(const Kv8Pages& c, int entry, int p
   return (long long)page * c.nkv * c.page_size + (pos - logical * c.page_size);
 }
 
-// A group of LANES lanes (a power of two, at least D / 8) takes a head's vector; a lane holds four pairs
-// (a[i], b[i]) that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others
-// pair up (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 8, so four pairs are two
-// stretches of four elements.
-template <typename T, int LANES>
+// E consecutive elements (4 or 8)
+template <int E, typename T> __device__ __forceinline__ void load_some(const T* src, float* out) {
+  if constexpr (E == 8) load8(src, out); else load4(src, out);
+}
+template <int E> __device__ __forceinline__ void store_some(bf16* dst, const float* v) {
+  if constexpr (E == 8) store8(dst, v); else store4(dst, v);
+}
+
+// A group of LANES lanes (a power of two, at least D / 2E) takes a head's vector; a lane holds E pairs (a[i], b[i])
+// that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others pair up
+// (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 2E, so E pairs are two stretches of E elements.
+// E = 8 where rows and R allow 16-byte loads of bfloat16 (4,096 tokens of 32 + 16 heads of 128: 34.6 us with E = 4, whose
+// instructions were the limit), else 4.  Queries are not measured for a scale, values not normalised.
+template <typename T, int LANES, int E>
 __global__ void __launch_bounds__(128)
 kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__ q_out, int nq, const T* __restrict__ k,
                  long long k_stride, const T* __restrict__ v, long long v_stride, const float* __restrict__ q_weight,
@@ -53,134 +62,176 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   const int token = blockIdx.x;
   const int lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES;
   const int warp = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = (blockDim.x >> 5) * gridDim.y;
+  const unsigned group = LANES == 32 ? 0xffffffffu : ((1u << LANES % 32) - 1u) << (sub * LANES);
   const int D = c.dim;
-  const bool mine = 8 * l < D;                   // lanes past the vector only take part in the sums
-  const int pair = 4 * l, half = rot >> 1;
+  const bool mine = 2 * E * l < D;               // lanes past the vector only take part in the sums
+  const int pair = E * l, half = rot >> 1;
   const bool turns = pair < half;
   const int ia = turns ? pair : rot + (pair - half), ib = turns ? pair + half : rot + ((D - rot) >> 1) + (pair - half);
   pdl_wait();
   const int pos = positions[token];
   const long long row = k == nullptr ? -1 : kv8_row(c, token_entry[token], pos, status, threadIdx.x == 0 && blockIdx.y == 0);
-  float cs[4], sn[4];
+  float cs[E], sn[E];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) { cs[e] = 1.f; sn[e] = 0.f; }
+  for (int e = 0; e < E; ++e) { cs[e] = 1.f; sn[e] = 0.f; }
   if (turns && mine) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 both = table[(size_t)token * half + pair + e];
-      cs[e] = both.x;
-      sn[e] = both.y;
+    for (int e = 0; e < E; e += 2) {
+      const float4 both = *reinterpret_cast<const float4*>(table + (size_t)token * half + pair + e);
+      cs[e] = both.x; sn[e] = both.y;
+      cs[e + 1] = both.z; sn[e + 1] = both.w;
     }
   }
   const int heads = nq + (k == nullptr ? 0 : 2 * c.nkv);
-  // every lane of a warp makes every round: the sums below are over whole warps
-  for (int first = warp * HEADS; first < heads; first += warps * HEADS) {
-    const int head = first + sub;
+  const T* q_row = q + (size_t)token * q_stride;
+  const T* k_row = k + (size_t)token * k_stride;
+  const T* v_row = v + (size_t)token * v_stride;
+  auto source = [&](int head) -> const T* {
+    return head < nq ? q_row + (size_t)head * D : head < nq + c.nkv ? k_row + (size_t)(head - nq) * D : v_row + (size_t)(head - nq - c.nkv) * D;
+  };
+  float a[E], b[E], next_a[E], next_b[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) { next_a[e] = 0.f; next_b[e] = 0.f; }
+  int head = warp * HEADS + sub;
+  auto fetch = [&](int h) {
+    if (mine && h < heads) {
+      const T* x = source(h);
+      load_some<E>(x + ia, next_a);
+      load_some<E>(x + ib, next_b);
+    }
+  };
+  fetch(head);
+  for (; head < heads; head += warps * HEADS) {             // the same for a group's lanes
     const bool is_q = head < nq, is_k = !is_q && head < nq + c.nkv;
-    const bool on = mine && head < heads && (is_q || row >= 0);
-    float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    const int kvh = is_q ? 0 : (is_k ? head - nq : head - nq - c.nkv);
-    if (on) {
-      const T* x = is_q ? q + (size_t)token * q_stride + (size_t)head * D
-                        : (is_k ? k + (size_t)token * k_stride : v + (size_t)token * v_stride) + (size_t)kvh * D;
-      load4(x + ia, a);
-      load4(x + ib, b);
-    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) { a[e] = next_a[e]; b[e] = next_b[e]; }
+    fetch(head + warps * HEADS);
     const float* w = is_q ? q_weight : (is_k ? k_weight : nullptr);
-    float ss = 0.f;
+    if (w != nullptr) {
+      float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ss += a[e] * a[e] + b[e] * b[e];
+      for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w != nullptr && on) {
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
       const float inv = rsqrtf(ss / (float)D + eps);
-      float wa[4], wb[4];
-      load4(w + ia, wa);
-      load4(w + ib, wb);
+      if (mine) {
+        float wa[E], wb[E];
+        load_some<E>(w + ia, wa);
+        load_some<E>(w + ib, wb);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { a[e] = a[e] * inv * wa[e]; b[e] = b[e] * inv * wb[e]; }
-    }
-    if (is_q || is_k) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = a[e] * cs[e] - b[e] * sn[e], y = b[e] * cs[e] + a[e] * sn[e];
-        if (turns) { a[e] = x; b[e] = y; }        // 0 * inf is not 0: what does not turn is left alone
+        for (int e = 0; e < E; ++e) { a[e] = a[e] * inv * wa[e]; b[e] = b[e] * inv * wb[e]; }
       }
+    }
+    if ((is_q || is_k) && turns) {                          // 0 * inf is not 0: what does not turn is left alone
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float x = a[e] * cs[e] - b[e] * sn[e], y = b[e] * cs[e] + a[e] * sn[e];
+        a[e] = x;
+        b[e] = y;
+      }
+    }
+    if (is_q) {
+      if (mine) {
+        bf16* dst = q_out + ((size_t)token * nq + head) * D;
+        store_some<E>(dst + ia, a);
+        store_some<E>(dst + ib, b);
+      }
+      continue;
     }
     unsigned big = 0u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < E; ++e)
       big = max(big, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-    if (!on) continue;
-    if (is_q) {
-      bf16* dst = q_out + ((size_t)token * nq + head) * D;
-      store4(dst + ia, a);
-      store4(dst + ib, b);
-      continue;
-    }
+    for (int o = LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(group, big, o));
+    if (!mine || row < 0) continue;
     const bool finite = big < 0x7f800000u;
     const int e8 = finite ? kv8_exponent(big) : 0;
     const float down = __int_as_float((127 - e8) << 23);
-    unsigned ca = 0u, cb = 0u;
-    if (finite) {
-      ca = (unsigned)kv8_codes(a[0] * down, a[1] * down) | (unsigned)kv8_codes(a[2] * down, a[3] * down) << 16;
-      cb = (unsigned)kv8_codes(b[0] * down, b[1] * down) | (unsigned)kv8_codes(b[2] * down, b[3] * down) << 16;
-    }
+    const int kvh = is_k ? head - nq : head - nq - c.nkv;
     const size_t at = (size_t)row + (size_t)kvh * c.page_size;
     unsigned char* dst = (is_k ? c.k : c.v) + at * D;
-    *reinterpret_cast<unsigned*>(dst + ia) = ca;
-    *reinterpret_cast<unsigned*>(dst + ib) = cb;
+    unsigned codes[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      codes[e / 4] = !finite ? 0u : (unsigned)kv8_codes(a[e] * down, a[e + 1] * down) | (unsigned)kv8_codes(a[e + 2] * down, a[e + 3] * down) << 16;
+      codes[E / 4 + e / 4] = !finite ? 0u : (unsigned)kv8_codes(b[e] * down, b[e + 1] * down) | (unsigned)kv8_codes(b[e + 2] * down, b[e + 3] * down) << 16;
+    }
+    if constexpr (E == 8) {
+      *reinterpret_cast<uint2*>(dst + ia) = make_uint2(codes[0], codes[1]);
+      *reinterpret_cast<uint2*>(dst + ib) = make_uint2(codes[2], codes[3]);
+    } else {
+      *reinterpret_cast<unsigned*>(dst + ia) = codes[0];
+      *reinterpret_cast<unsigned*>(dst + ib) = codes[1];
+    }
     if (l == 0) (is_k ? c.ks : c.vs)[at] = (unsigned char)(finite ? e8 + KV8_BIAS : KV8_NAN);
   }
 }
 
-__device__ __forceinline__ void kv8_store16(bf16* dst, const float* v) { store8(dst, v); store8(dst + 8, v + 8); }
-__device__ __forceinline__ void kv8_store16(float* dst, const float* v) { store8(dst, v); store8(dst + 8, v + 8); }
+// 16 bytes of output from as many codes, times their scale
+__device__ __forceinline__ void kv8_put(bf16* dst, uint2 codes, float scale) {
+  float out[8];
+  unsigned h[4];
+  kv8_halves(codes.x, h[0], h[1]);
+  kv8_halves(codes.y, h[2], h[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    out[2 * i] = f.x * scale;
+    out[2 * i + 1] = f.y * scale;
+  }
+  store8(dst, out);
+}
+__device__ __forceinline__ void kv8_put(float* dst, unsigned codes, float scale) {
+  unsigned h[2];
+  kv8_halves(codes, h[0], h[1]);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[0])), b = __half22float2(*reinterpret_cast<const __half2*>(&h[1]));
+  *reinterpret_cast<float4*>(dst) = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
+}
 
-// A thread takes 16 codes of a token's key vector and the 16 of its value vector.
+// A warp takes a token: neighbouring lanes write neighbouring 16 bytes of its rows (with 16 codes a thread, whose 64
+// bytes of output lay apart, 73,728 tokens of 4 heads of 64 in 32 bits took 25.6 us).
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv8_read_kernel(Kv8Pages c, const int* __restrict__ positions, const int* __restrict__ token_entry, T* __restrict__ k_out,
                 T* __restrict__ v_out, int tokens, int* status) {
+  constexpr int N = 16 / sizeof(T);             // codes a lane takes at a time
+  using Codes = std::conditional_t<N == 8, uint2, unsigned>;
   pdl_trigger();
   pdl_wait();
-  const int chunks = c.dim >> 4, per_token = c.nkv * chunks;
-  const long long unit = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long token = unit / per_token;
+  const int lane = threadIdx.x & 31;
+  const long long token = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (token >= tokens) return;
-  const int rest = (int)(unit - token * per_token), head = rest / chunks, chunk = rest - head * chunks;
-  const long long row = kv8_row(c, token_entry[token], positions[token], status, rest == 0);
-  uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-  float scale[2] = {0.f, 0.f};
-  if (row >= 0) {
-    const size_t at = (size_t)row + (size_t)head * c.page_size;
-    raw[0] = __ldcs(reinterpret_cast<const uint4*>(c.k + at * c.dim) + chunk);
-    raw[1] = __ldcs(reinterpret_cast<const uint4*>(c.v + at * c.dim) + chunk);
-    scale[0] = kv8_scale(c.ks[at]);
-    scale[1] = kv8_scale(c.vs[at]);
-  }
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const unsigned words[4] = {raw[m].x, raw[m].y, raw[m].z, raw[m].w};
-    float out[16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned h = kv8_half2((unsigned short)(words[i >> 1] >> (16 * (i & 1))));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      out[2 * i] = f.x * scale[m];
-      out[2 * i + 1] = f.y * scale[m];
+  const long long row = kv8_row(c, token_entry[token], positions[token], status, lane == 0);
+  const int width = c.nkv * c.dim, step = 32 * N, heads_a_step = step / c.dim, rest = step - heads_a_step * c.dim;
+  int head = lane * N / c.dim, at = lane * N - head * c.dim;
+  T* k_row = k_out + (size_t)token * width;
+  T* v_row = v_out + (size_t)token * width;
+#pragma unroll 4
+  for (int i = lane * N; i < width; i += step) {
+    Codes k{}, v{};
+    float k_scale = 0.f, v_scale = 0.f;
+    if (row >= 0) {
+      const size_t place = (size_t)row + (size_t)head * c.page_size;
+      k = __ldcs(reinterpret_cast<const Codes*>(c.k + place * c.dim + at));
+      v = __ldcs(reinterpret_cast<const Codes*>(c.v + place * c.dim + at));
+      k_scale = kv8_scale(c.ks[place]);
+      v_scale = kv8_scale(c.vs[place]);
     }
-    kv8_store16((m ? v_out : k_out) + (size_t)token * per_token * 16 + (size_t)rest * 16, out);
+    kv8_put(k_row + i, k, k_scale);
+    kv8_put(v_row + i, v, v_scale);
+    head += heads_a_step;
+    at += rest;
+    if (at >= c.dim) { at -= c.dim; ++head; }
   }
 }
 
-template <typename T>
+template <typename T, int E>
 int kv8_write_typed(const void* q, long long q_stride, bf16* q_out, int nq, const void* k, long long k_stride, const void* v,
                     long long v_stride, const float* q_weight, const float* k_weight, float eps, const float2* table, int rot,
                     const int* positions, const int* token_entry, const Kv8Pages& c, int tokens, int* status, cudaStream_t stream) {
-  const int lanes = c.dim <= 16 ? 2 : c.dim <= 32 ? 4 : c.dim <= 64 ? 8 : c.dim <= 128 ? 16 : 32;
+  int lanes = 1;
+  while (lanes * 2 * E < c.dim) lanes *= 2;
   const int heads_a_warp = 32 / lanes, heads = nq + (k == nullptr ? 0 : 2 * c.nkv);
   if (heads == 0) return 0;
   const int rounds = (heads + 4 * heads_a_warp - 1) / (4 * heads_a_warp);      // of a block of four warps over a token's heads
@@ -192,11 +243,12 @@ int kv8_write_typed(const void* q, long long q_stride, bf16* q_out, int nq, cons
                                (const T*)v, v_stride, q_weight, k_weight, eps, table, rot, positions, token_entry, c, status);
   };
   switch (lanes) {
-    case 2: return launch(kv8_write_kernel<T, 2>);
-    case 4: return launch(kv8_write_kernel<T, 4>);
-    case 8: return launch(kv8_write_kernel<T, 8>);
-    case 16: return launch(kv8_write_kernel<T, 16>);
-    default: return launch(kv8_write_kernel<T, 32>);
+    case 1: return launch(kv8_write_kernel<T, 1, E>);
+    case 2: return launch(kv8_write_kernel<T, 2, E>);
+    case 4: return launch(kv8_write_kernel<T, 4, E>);
+    case 8: return launch(kv8_write_kernel<T, 8, E>);
+    case 16: return launch(kv8_write_kernel<T, 16, E>);
+    default: return launch(kv8_write_kernel<T, 32, E>);
   }
 }
 
@@ -228,12 +280,17 @@ FE_EXPORT int fe_kv8_write(const void* q, long long q_stride, void* q_out, int n
   if (dtype != FE_DTYPE_F32 && dtype != FE_DTYPE_BF16) return FE_ERR_BAD_DTYPE;
   const uintptr_t rows = dtype == FE_DTYPE_F32 ? 15 : 7;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & rows || (q_stride | k_stride | v_stride) % 4) return FE_ERR_BAD_ALIGN;
-  if (((uintptr_t)q_out & 7) || (((uintptr_t)q_weight | (uintptr_t)k_weight) & 15) || ((uintptr_t)table & 7)) return FE_ERR_BAD_ALIGN;
-  const int done = dtype == FE_DTYPE_F32
-                       ? kv8_write_typed<float>(q, q_stride, (bf16*)q_out, nq, k, k_stride, v, v_stride, q_weight, k_weight, eps,
-                                                (const float2*)table, rot, positions, token_entry, c, tokens, status, stream)
-                       : kv8_write_typed<bf16>(q, q_stride, (bf16*)q_out, nq, k, k_stride, v, v_stride, q_weight, k_weight, eps,
-                                               (const float2*)table, rot, positions, token_entry, c, tokens, status, stream);
+  if (((uintptr_t)q_out & 7) || (((uintptr_t)q_weight | (uintptr_t)k_weight) & 15) || ((uintptr_t)table & 15)) return FE_ERR_BAD_ALIGN;
+  // 16-byte loads of eight elements
+  const bool wide = rot % 16 == 0 && !((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & 15) || (q_stride | k_stride | v_stride) % 8);
+  auto write = [&](auto kind, auto each) {
+    using T = decltype(kind);
+    return kv8_write_typed<T, decltype(each)::value>(q, q_stride, (bf16*)q_out, nq, k, k_stride, v, v_stride, q_weight, k_weight, eps,
+                                                     (const float2*)table, rot, positions, token_entry, c, tokens, status, stream);
+  };
+  using Eight = std::integral_constant<int, 8>;
+  using Four = std::integral_constant<int, 4>;
+  const int done = dtype == FE_DTYPE_F32 ? (wide ? write(float(), Eight()) : write(float(), Four())) : (wide ? write(bf16(), Eight()) : write(bf16(), Four()));
   return done ? done : fe_last_error();
 }
 
@@ -248,7 +305,7 @@ FE_EXPORT int fe_kv8_read(const void* k_cache, const void* v_cache, const void* 
   if (rc) return rc;
   if (dtype != FE_DTYPE_F32 && dtype != FE_DTYPE_BF16) return FE_ERR_BAD_DTYPE;
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return FE_ERR_BAD_ALIGN;
-  const long long blocks = ((long long)tokens * nkv * (dim / 16) + 255) / 256;
+  const long long blocks = ((long long)tokens + 7) / 8;
   if (blocks > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
   const dim3 grid((unsigned)blocks);
   const int done = dtype == FE_DTYPE_F32

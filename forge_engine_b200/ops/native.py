@@ -1921,45 +1921,62 @@ def kv8_lib(head_dim: int):
     return got
 
 
-def _kv8_refuse(unless: bool, message: str) -> None:
-    if not unless:
-        raise UnsupportedShapeError(message)
-
-
 def _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status) -> tuple:
     """(pages, kv heads, page size, head size) after the checks of types and shapes that every call over an 8-bit cache makes."""
-    _kv8_refuse(k_cache.dtype == v_cache.dtype == KV8_CODES and k_scale.dtype == v_scale.dtype == KV8_SCALES,
-                "an 8-bit cache holds float8_e4m3fn codes and float8_e8m0fnu scales")
-    shape = tuple(k_cache.shape)
-    _kv8_refuse(len(shape) == 4 and tuple(v_cache.shape) == shape and tuple(k_scale.shape) == tuple(v_scale.shape) == shape[:3],
-                "an 8-bit cache is [pages, kv heads, page size, head size] codes and [pages, kv heads, page size] scales")
-    _kv8_refuse(kv8_takes(shape[3]), f"head size {shape[3]}: the 8-bit cache takes multiples of 16 up to 256")
-    _kv8_refuse(shape[1] >= 1 and shape[2] >= 1, "an 8-bit cache has kv heads and pages of at least one token")
-    _kv8_refuse(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table is [entries, pages] int32")
-    _kv8_refuse(status.dtype == torch.int32 and status.numel() >= 1, "status is an int32 word")
+    if not (k_cache.dtype == v_cache.dtype == KV8_CODES and k_scale.dtype == v_scale.dtype == KV8_SCALES):
+        raise UnsupportedShapeError("an 8-bit cache holds float8_e4m3fn codes and float8_e8m0fnu scales")
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or not k_scale.shape == v_scale.shape == shape[:3]:
+        raise UnsupportedShapeError("an 8-bit cache is [pages, kv heads, page size, head size] codes and [pages, kv heads, page size] scales")
+    if not kv8_takes(shape[3]):
+        raise UnsupportedShapeError(f"head size {shape[3]}: the 8-bit cache takes multiples of 16 up to 256")
+    if shape[1] < 1 or shape[2] < 1:
+        raise UnsupportedShapeError("an 8-bit cache has kv heads and pages of at least one token")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise UnsupportedShapeError("block_table is [entries, pages] int32")
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise UnsupportedShapeError("status is an int32 word")
     return shape
 
 
-def _kv8_device(first: torch.Tensor, *others, rows=()) -> None:
-    """Everything on one CUDA device, and dense but for ``rows``."""
-    for t in (first, *others):
-        if t is not None and t.numel():
-            _dense(t, "every tensor of a call over the 8-bit cache but k, v and q")
-    for t in (first, *others, *rows):
-        if t is not None and t.device != first.device:
-            raise UnsupportedShapeError(f"tensors on {first.device} and {t.device}: a call works on one device")
+def _kv8_device(dense: tuple, rows: tuple) -> int:
+    """The CUDA device that all tensors lie on; ``dense`` ones have to be dense."""
+    index = dense[0].get_device()
+    for t in dense:
+        if t is not None:
+            if t.get_device() != index:
+                raise UnsupportedShapeError("tensors on several devices: a call works on one")
+            if not t.is_contiguous():
+                raise UnsupportedShapeError("every tensor of a call over the 8-bit cache but k, v and q must be dense")
+    for t in rows:
+        if t is not None and t.get_device() != index:
+            raise UnsupportedShapeError("tensors on several devices: a call works on one")
+    if index < 0:
+        raise CUDAUnavailableError("the 8-bit cache lives on the CUDA device")
+    return index
 
 
 def _kv8_rows(t: torch.Tensor, n: int, width: int, name: str) -> int:
     """The distance of the rows of ``t`` [n, width]."""
-    _kv8_refuse(t.dim() == 2 and tuple(t.shape) == (n, width) and (width <= 1 or t.stride(1) == 1),
-                f"{name} must be [{n}, {width}] with neighbouring elements side by side, got {tuple(t.shape)}")
-    return int(t.stride(0)) if n > 1 else width
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise UnsupportedShapeError(f"{name} must be [{n}, {width}] with neighbouring elements side by side, got {tuple(t.shape)}")
+    return t.stride(0) if n > 1 else width
 
 
-def _kv8_places(positions: torch.Tensor, token_entry: torch.Tensor, n: int) -> None:
-    for t, name in ((positions, "positions"), (token_entry, "token_entry")):
-        _kv8_refuse(t.dtype == torch.int32 and t.numel() == n, f"{name} must hold {n} int32 numbers")
+def _kv8_places(positions: torch.Tensor, token_entry: torch.Tensor) -> int:
+    n = positions.numel()
+    if positions.dtype != torch.int32 or token_entry.dtype != torch.int32 or token_entry.numel() != n:
+        raise UnsupportedShapeError("positions and token_entry hold one int32 number a token each")
+    return n
+
+
+def _kv8_call(index: int, fn, args: tuple, what: str) -> None:
+    """``fn`` with ``args`` and the current stream of device ``index``."""
+    if torch.cuda.current_device() == index:
+        check(fn(*args, stream()), what)
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, stream()), what)
 
 
 def kv8_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.Tensor, token_entry: torch.Tensor,
@@ -1983,34 +2000,39 @@ def kv8_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.T
 
     A position outside the block table or a missing page sets a bit of ``status`` and writes nothing."""
     num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
-    _kv8_refuse((k is None) == (v is None) and (q is None) == (q_out is None), "kv8_write: k goes with v, and q with q_out")
     some = q if k is None else k
-    _kv8_refuse(some is not None, "kv8_write: nothing to write")
-    n = positions.numel()
-    _kv8_places(positions, token_entry, n)
+    if (k is None) != (v is None) or (q is None) != (q_out is None) or some is None:
+        raise UnsupportedShapeError("kv8_write: k goes with v and q with q_out, and one of the two pairs is there")
+    n = _kv8_places(positions, token_entry)
     k_stride = v_stride = q_stride = heads = 0
+    dtype = some.dtype
     if k is not None:
         k_stride, v_stride = _kv8_rows(k, n, nkv * d, "k"), _kv8_rows(v, n, nkv * d, "v")
+        if v.dtype != dtype:
+            raise UnsupportedShapeError("k, v and q are of one type")
     if q is not None:
         heads = q.shape[-1] // d
         q_stride = _kv8_rows(q, n, heads * d, "q")
-        _kv8_refuse(q_out.dtype == torch.bfloat16 and q_out.shape == q.shape, "q_out must be bfloat16 of q's shape")
-    _kv8_refuse(all(t is None or t.dtype == some.dtype for t in (k, v, q)), "k, v and q are of one type")
+        if q.dtype != dtype or q_out.dtype != torch.bfloat16 or q_out.shape != q.shape:
+            raise UnsupportedShapeError("k, v and q are of one type, and q_out is bfloat16 of q's shape")
     some_code = code(some)
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _kv8_refuse(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (d,)), f"{name} must be 32-bit, [{d}]")
-    _kv8_refuse(table is None or (table.dtype == torch.float32 and table.dim() == 3 and table.shape[0] == n and table.shape[2] == 2),
-                f"table must be 32-bit, [{n}, pairs, 2]")
-    rot = 0 if table is None else 2 * int(table.shape[1])
-    _kv8_refuse(rot <= d and rot % 8 == 0, f"{rot} rotated elements: a multiple of 8 up to the head size {d}")
-    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, q_out, q_norm, k_norm, table,
-                rows=(k, v, q))
-    with torch.cuda.device(k_cache.device):
-        check(lib().fe_kv8_write(ptr(q), q_stride, ptr(q_out), heads, ptr(k), k_stride, ptr(v), v_stride, some_code, ptr(q_norm),
-                                 ptr(k_norm), float(eps), ptr(table) if rot else None, rot, ptr(positions), ptr(token_entry),
-                                 ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table),
-                                 block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, d, n, ptr(status),
-                                 stream()), "kv8_write")
+    for t in (q_norm, k_norm):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != d):
+            raise UnsupportedShapeError(f"q_norm and k_norm are 32-bit, [{d}]")
+    rot = 0
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 3 or table.shape[0] != n or table.shape[2] != 2:
+            raise UnsupportedShapeError(f"table must be 32-bit, [{n}, pairs, 2]")
+        rot = 2 * table.shape[1]
+        if rot > d or rot % 8:
+            raise UnsupportedShapeError(f"{rot} rotated elements: a multiple of 8 up to the head size {d}")
+    index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, q_out, q_norm, k_norm, table),
+                        (k, v, q))
+    _kv8_call(index, lib().fe_kv8_write,
+              (ptr(q), q_stride, ptr(q_out), heads, ptr(k), k_stride, ptr(v), v_stride, some_code, ptr(q_norm), ptr(k_norm), eps,
+               ptr(table) if rot else None, rot, ptr(positions), ptr(token_entry), k_cache.data_ptr(), v_cache.data_ptr(),
+               k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[0], block_table.shape[1], page_size,
+               num_pages, nkv, d, n, status.data_ptr()), "kv8_write")
 
 
 def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -2020,24 +2042,22 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
     lies at ``positions[n]`` of entry ``token_entry[n]``.  A position outside the block table or a missing page sets a
     bit of ``status`` and gives zeros."""
     num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
-    n = positions.numel()
-    _kv8_places(positions, token_entry, n)
-    _kv8_refuse(k_out.dtype == v_out.dtype and tuple(k_out.shape) == tuple(v_out.shape) == (n, nkv, d),
-                f"k_out and v_out must be [{n}, {nkv}, {d}] of one type")
+    n = _kv8_places(positions, token_entry)
+    if k_out.dtype != v_out.dtype or k_out.shape != (n, nkv, d) or v_out.shape != (n, nkv, d):
+        raise UnsupportedShapeError(f"k_out and v_out must be [{n}, {nkv}, {d}] of one type")
     out_code = code(k_out)
-    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, k_out, v_out)
-    with torch.cuda.device(k_cache.device):
-        check(lib().fe_kv8_read(ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table), block_table.shape[0],
-                                block_table.shape[1], page_size, num_pages, nkv, d, ptr(positions), ptr(token_entry), ptr(k_out),
-                                ptr(v_out), out_code, n, ptr(status), stream()), "kv8_read")
+    index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, positions, token_entry, k_out, v_out), ())
+    _kv8_call(index, lib().fe_kv8_read,
+              (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+               block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, d, ptr(positions), ptr(token_entry), ptr(k_out),
+               ptr(v_out), out_code, n, status.data_ptr()), "kv8_read")
 
 
 def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window: int | None = None, keep_first: int = 0) -> tuple:
-    """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries: (key tiles a
+    """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries (tuples): (key tiles a
     block takes of an entry with at most 16 rows, such blocks of the longest one, and both for the other entries);
     a count of 0: there is no such entry.  Layers of one geometry share it."""
-    return _kv8_plan(tuple((int(start), int(count)) for start, count in entries), int(num_q_heads) // int(num_kv_heads),
-                     int(num_kv_heads), int(head_dim), int(window or 0), int(keep_first or 0))
+    return _kv8_plan(tuple(entries), num_q_heads // num_kv_heads, num_kv_heads, head_dim, window or 0, keep_first or 0)
 
 
 def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, tile: int) -> int:
@@ -2095,27 +2115,30 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     the last ``window`` of them and the first ``keep_first`` of the sequence.  ``out`` [N, heads * D] (bfloat16, dense); rows
     of no entry are left as they are.  ``plan``: ``kv8_plan`` of these entries.  32-bit scores, softmax and sums."""
     num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
-    n_entries, max_new, window, keep_first = int(n_entries), int(max_new), int(window or 0), int(keep_first or 0)
-    n = q.shape[0]
-    _kv8_refuse(num_q_heads >= 1 and num_q_heads % nkv == 0, f"{num_q_heads} heads over {nkv} kv heads")
+    window, keep_first, n = window or 0, keep_first or 0, q.shape[0]
+    if num_q_heads < 1 or num_q_heads % nkv:
+        raise UnsupportedShapeError(f"{num_q_heads} heads over {nkv} kv heads")
     q_stride = _kv8_rows(q, n, num_q_heads * d, "q")
-    _kv8_refuse(q.dtype == out.dtype == torch.bfloat16 and out.shape == q.shape, "q and out are bfloat16 of one shape")
-    _kv8_refuse(n_entries >= 0 and max_new >= 0 and window >= 0 and keep_first >= 0, "attention_kv8: no negative sizes")
-    _kv8_refuse(cu_tokens.dtype == starts.dtype == torch.int32 and cu_tokens.numel() > n_entries and starts.numel() >= n_entries,
-                "cu_tokens holds entries + 1 int32 numbers, starts one an entry")
-    _kv8_refuse(block_table.shape[0] >= n_entries, "attention_kv8: a block table row per entry")
-    _kv8_refuse(scale > 0, "attention_kv8: the scale is positive")
-    _kv8_device(k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out, rows=(q,))
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape:
+        raise UnsupportedShapeError("q and out are bfloat16 of one shape")
+    if n_entries < 0 or max_new < 0 or window < 0 or keep_first < 0 or not scale > 0:
+        raise UnsupportedShapeError("attention_kv8: no negative sizes, and a positive scale")
+    if (cu_tokens.dtype != torch.int32 or starts.dtype != torch.int32 or cu_tokens.numel() <= n_entries or starts.numel() < n_entries
+            or block_table.shape[0] < n_entries):
+        raise UnsupportedShapeError("cu_tokens holds entries + 1 int32 numbers, starts one an entry, block_table a row")
+    index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out), (q,))
     single_span, single_spans, portion_span, portion_spans = plan
     groups = num_q_heads // nkv
     if max_new * groups <= KV8_SINGLE_ROWS:
         portion_spans = 0
     fn, size = kv8_lib(d)
-    with torch.cuda.device(q.device):
+    workspace = None
+    if single_spans > 1 or portion_spans > 1:
         # the pieces of a cut entry meet in a buffer of the call's own: calls on other streams, and captured ones, have theirs
         numbers = max(size(0, n_entries, nkv, groups, n, single_spans), size(1, n_entries, nkv, groups, n, portion_spans))
-        workspace = torch.empty(numbers, dtype=torch.float32, device=q.device) if numbers else None
-        check(fn(ptr(q), q_stride, ptr(out), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(block_table),
-                 block_table.shape[1], page_size, num_pages, nkv, groups, ptr(cu_tokens), ptr(starts), n_entries, n, window,
-                 keep_first, float(scale), single_span, single_spans, portion_span, portion_spans, ptr(workspace), ptr(status),
-                 stream()), "attention_kv8")
+        workspace = torch.empty(numbers, dtype=torch.float32, device=q.device)
+    _kv8_call(index, fn,
+              (q.data_ptr(), q_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+               block_table.data_ptr(), block_table.shape[1], page_size, num_pages, nkv, groups, cu_tokens.data_ptr(),
+               starts.data_ptr(), n_entries, n, window, keep_first, scale, single_span, single_spans, portion_span,
+               portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")
