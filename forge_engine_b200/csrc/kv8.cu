@@ -42,6 +42,33 @@ __device__ __forceinline__ long long kv8_row(const Kv8Pages& c, int entry, int p
 template <int E, typename T> __device__ __forceinline__ void load_some(const T* src, float* out) {
   if constexpr (E == 8) load8(src, out); else load4(src, out);
 }
+// E elements as they lie in memory: what is asked for a round ahead waits in as few registers as it can
+template <int E, typename T> struct Held {
+  static constexpr int WORDS = E * (int)sizeof(T) / 4;
+  unsigned w[WORDS];
+  __device__ __forceinline__ void load(const T* src) {
+    if constexpr (WORDS == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(src);
+      w[0] = x.x; w[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 x = reinterpret_cast<const uint4*>(src)[i / 4];
+        w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void numbers(float* out) const {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (sizeof(T) == 4) out[i] = __uint_as_float(w[i]);
+      else {
+        out[2 * i] = __uint_as_float(w[i] << 16);
+        out[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+};
 template <int E> __device__ __forceinline__ void store_some(bf16* dst, const float* v) {
   if constexpr (E == 8) store8(dst, v); else store4(dst, v);
 }
@@ -52,7 +79,7 @@ template <int E> __device__ __forceinline__ void store_some(bf16* dst, const flo
 // E = 8 where rows and R allow 16-byte loads of bfloat16 (4,096 tokens of 32 + 16 heads of 128: 34.6 us with E = 4, whose
 // instructions were the limit), else 4.  Queries are not measured for a scale, values not normalised.
 template <typename T, int LANES, int E>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 8)
 kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__ q_out, int nq, const T* __restrict__ k,
                  long long k_stride, const T* __restrict__ v, long long v_stride, const float* __restrict__ q_weight,
                  const float* __restrict__ k_weight, float eps, const float2* __restrict__ table, int rot,
@@ -69,8 +96,6 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   const bool turns = pair < half;
   const int ia = turns ? pair : rot + (pair - half), ib = turns ? pair + half : rot + ((D - rot) >> 1) + (pair - half);
   pdl_wait();
-  const int pos = positions[token];
-  const long long row = k == nullptr ? -1 : kv8_row(c, token_entry[token], pos, status, threadIdx.x == 0 && blockIdx.y == 0);
   float cs[E], sn[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { cs[e] = 1.f; sn[e] = 0.f; }
@@ -89,22 +114,23 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   auto source = [&](int head) -> const T* {
     return head < nq ? q_row + (size_t)head * D : head < nq + c.nkv ? k_row + (size_t)(head - nq) * D : v_row + (size_t)(head - nq - c.nkv) * D;
   };
-  float a[E], b[E], next_a[E], next_b[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) { next_a[e] = 0.f; next_b[e] = 0.f; }
+  Held<E, T> held_a{}, held_b{};
   int head = warp * HEADS + sub;
   auto fetch = [&](int h) {
     if (mine && h < heads) {
       const T* x = source(h);
-      load_some<E>(x + ia, next_a);
-      load_some<E>(x + ib, next_b);
+      held_a.load(x + ia);
+      held_b.load(x + ib);
     }
   };
   fetch(head);
+  // the first rows are on their way before the place is looked up
+  const long long row = k == nullptr ? -1 : kv8_row(c, token_entry[token], positions[token], status, threadIdx.x == 0 && blockIdx.y == 0);
   for (; head < heads; head += warps * HEADS) {             // the same for a group's lanes
     const bool is_q = head < nq, is_k = !is_q && head < nq + c.nkv;
-#pragma unroll
-    for (int e = 0; e < E; ++e) { a[e] = next_a[e]; b[e] = next_b[e]; }
+    float a[E], b[E];
+    held_a.numbers(a);
+    held_b.numbers(b);
     fetch(head + warps * HEADS);
     const float* w = is_q ? q_weight : (is_k ? k_weight : nullptr);
     if (w != nullptr) {
