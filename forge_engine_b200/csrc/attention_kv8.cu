@@ -270,6 +270,39 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
   for (int h = 0; h < 2; ++h) s.l[h] = s.l[h] * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
 }
 
+// The codes of a step's 32 keys and values; lane l knows the row of key l in its cache (-1: none, zeros).  ALL: every key
+// has one.
+template <bool ALL>
+__device__ __forceinline__ void copy_step(const Kv8Attention& p, unsigned char* stage, int mine, int lane) {
+  if constexpr (32 % CHUNKS == 0) {
+    // a lane's pieces lie STRIDE rows apart; their places in the stage differ by a constant, in the values' exchange of
+    // pieces by a constant bit pattern
+    constexpr int STRIDE = 32 / CHUNKS;
+    const int row0 = lane / CHUNKS, c = lane % CHUNKS;
+    const unsigned char* k = p.k + c * 16;
+    const unsigned char* v = p.v + c * 16;
+    const unsigned kd = smem_addr(stage) + row0 * D + key_piece(row0, c) * 16, vd = smem_addr(stage) + MATRIX + row0 * D + value_piece(row0, c) * 16;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+      const int from = __shfl_sync(0xffffffffu, mine, row0 + STRIDE * j);
+      const size_t offset = (size_t)(unsigned)(ALL ? from : max(from, 0)) * D;
+      const unsigned turn = D % 128 == 0 ? (unsigned)((j * STRIDE / 2) & 3) << 5 : D % 64 == 0 ? (unsigned)((j * STRIDE / 2) & 3) << 4 : 0u;
+      const int bytes = ALL || from >= 0 ? 16 : 0;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(kd + j * STRIDE * D), "l"(k + offset), "r"(bytes));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((vd ^ turn) + j * STRIDE * D), "l"(v + offset), "r"(bytes));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+      const int u = lane + 32 * j, row = u / CHUNKS, c = u - row * CHUNKS;
+      const int from = __shfl_sync(0xffffffffu, mine, row);
+      const size_t offset = (size_t)max(from, 0) * D + c * 16;
+      cp_async16(stage + row * D + key_piece(row, c) * 16, p.k + offset, from >= 0);
+      cp_async16(stage + MATRIX + row * D + value_piece(row, c) * 16, p.v + offset, from >= 0);
+    }
+  }
+}
+
 // PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of its tiles.  Otherwise it takes the (at most
 // 16) rows of an entry, and warp w the keys 32 w .. 32 w + 31 of every tile; the warps' sums join at the end.
 // A warp goes its own way: it copies its keys into a ring of its own, a step ahead, and waits for nobody (with a ring of the
@@ -339,14 +372,8 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
       page = look_up(i + 2);
       const int mine = there ? (int)at : -1;             // the launcher holds the rows of a cache to 31 bits
       unsigned char* stage = ring + ((i + 1) & 1) * STAGE;
-#pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) {
-        const int u = lane + 32 * j, row = u / CHUNKS, c = u - row * CHUNKS;
-        const int from = __shfl_sync(0xffffffffu, mine, row);
-        const size_t offset = (size_t)max(from, 0) * D + c * 16;
-        cp_async16(stage + row * D + key_piece(row, c) * 16, p.k + offset, from >= 0);
-        cp_async16(stage + MATRIX + row * D + value_piece(row, c) * 16, p.v + offset, from >= 0);
-      }
+      if (__all_sync(0xffffffffu, there)) copy_step<true>(p, stage, mine, lane);
+      else copy_step<false>(p, stage, mine, lane);
     }
     cp_async_commit();
     if (i < 0) {
