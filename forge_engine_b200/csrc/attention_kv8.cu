@@ -36,7 +36,7 @@ constexpr int ROWS = 16;                // rows a warp takes: the m of one mma
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int STAGES = 2;
 constexpr int MATRIX = STEP * D;        // bytes of one matrix of a stage
-constexpr int STAGE = 2 * MATRIX + 3 * STEP * 4;      // codes, then of every key: 2^a, b and 2^-b
+constexpr int STAGE = 2 * MATRIX + STEP * 16;      // codes, then of every key: 2^a, b, 2^-b
 constexpr size_t RING = (size_t)WARPS * STAGES * STAGE;
 constexpr size_t JOIN = (size_t)WARPS * ROWS * (D + 2) * sizeof(float);
 constexpr size_t MMA_SMEM = RING > JOIN ? RING : JOIN;
@@ -189,7 +189,7 @@ __device__ __forceinline__ int value_column(int n, int c, int t) {
 __device__ __forceinline__ void take(const Queries& q, const unsigned char* stage, int key0, const Kv8Attention& p, bool clear,
                                      int pos_a, int pos_b, Sums& s, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  const float* of_key = reinterpret_cast<const float*>(stage + 2 * MATRIX);
+  const float4* of_key = reinterpret_cast<const float4*>(stage + 2 * MATRIX);
   float c[STEP / 8][4];
   float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -214,12 +214,11 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
       mma_f16(c[n], q.a[i], b0, b1);
     }
     // keys 8 n + 2 t and the next one
-    const float2 up = *reinterpret_cast<const float2*>(of_key + 8 * n + 2 * t);
-    const float2 add = *reinterpret_cast<const float2*>(of_key + STEP + 8 * n + 2 * t);
+    const float4 k0 = of_key[8 * n + 2 * t], k1 = of_key[8 * n + 2 * t + 1];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      c[n][2 * h] = fmaf(c[n][2 * h] * up.x, q.factor[h], add.x);
-      c[n][2 * h + 1] = fmaf(c[n][2 * h + 1] * up.y, q.factor[h], add.y);
+      c[n][2 * h] = fmaf(c[n][2 * h] * k0.x, q.factor[h], k0.y);
+      c[n][2 * h + 1] = fmaf(c[n][2 * h + 1] * k1.x, q.factor[h], k1.y);
     }
     if (!clear) {
 #pragma unroll
@@ -251,7 +250,7 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
     unsigned a[4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const float2 back = *reinterpret_cast<const float2*>(of_key + 2 * STEP + 16 * k + 8 * n + 2 * t);
+      const float2 back = make_float2(of_key[16 * k + 8 * n + 2 * t].z, of_key[16 * k + 8 * n + 2 * t + 1].z);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float w0 = exp2_fast(c[2 * k + n][2 * h] - base[h]), w1 = exp2_fast(c[2 * k + n][2 * h + 1] - base[h]);
@@ -303,11 +302,334 @@ __device__ __forceinline__ void copy_step(const Kv8Attention& p, unsigned char* 
   }
 }
 
+// A warp goes its own way through its keys: it copies them into a ring of its own, a step ahead, and waits for nobody (with
+// a ring of the block and a barrier a tile, 64 keys of one head took 1.7 us a block whatever else ran).  A lane looks after
+// one key of a step: its page, looked up two steps ahead, its place and its scales, asked for with the codes.
+struct WarpRing {
+  unsigned char* ring;
+  const Kv8Attention& p;
+  const int* table;
+  int kvh, key_lo, key_end, lane, page, k_scale, v_scale;
+  __device__ __forceinline__ WarpRing(unsigned char* ring, const Kv8Attention& p, const int* table, int kvh, int key_lo, int key_end, int lane)
+      : ring(ring), p(p), table(table), kvh(kvh), key_lo(key_lo), key_end(key_end), lane(lane), page(-1), k_scale(KV8_BIAS), v_scale(KV8_BIAS) {}
+  __device__ __forceinline__ unsigned char* stage(int i) const { return ring + (i & 1) * STAGE; }
+  __device__ __forceinline__ void look_up(int key0) { page = key_page(p, table, key0 + lane, key_end); }
+  // The scales of step i, asked for with its codes.  A key whose value is not finite counts as not finite itself.
+  __device__ __forceinline__ void put_scales(int i) const {
+    const bool bad = v_scale == KV8_NAN;
+    reinterpret_cast<float4*>(stage(i) + 2 * MATRIX)[lane] =
+        make_float4(kv8_scale(bad ? KV8_NAN : k_scale), bad ? 0.f : (float)(v_scale - KV8_BIAS),
+                    bad ? 1.f : __int_as_float((2 * KV8_BIAS - v_scale) << 23), 0.f);
+  }
+  // Ask for the codes and scales of step i, at positions from key0 on, and for the pages of the one after it.
+  __device__ __forceinline__ void ask(int i, int key0, int next_key0) {
+    const int key = key0 + lane;
+    long long at;
+    const bool there = key_row(p, page, kvh, key, &at);
+    if (!there) tell_missing(p, key, key_lo, key_end);
+    k_scale = v_scale = KV8_BIAS;
+    if (there) {
+      k_scale = __ldg(p.ks + at);
+      v_scale = __ldg(p.vs + at);
+    }
+    look_up(next_key0);
+    const int row = there ? (int)at : -1;             // the launcher holds the rows of a cache to 31 bits
+    if (__all_sync(0xffffffffu, there)) copy_step<true>(p, stage(i), row, lane);
+    else copy_step<false>(p, stage(i), row, lane);
+  }
+};
+
+// ---- up to eight rows, head sizes of whole 32s ----
+//
+// Keys stand on the side of 16 of a product and the rows on the side of 8, so a GQA group of up to eight heads wastes
+// nothing.  (Two eights of rows did not fit a thread's registers: 235 us for 48 windows of 15 rows, where the kernel of
+// 16 rows takes 87.)  Scores are products of 8-bit numbers, the codes as they lie in shared memory against two e4m3
+// numbers of a query element: a row times a power of two, rounded, and what the rounding left.  They hold bfloat16's 8
+// bits down to 2^-11 of the row's largest element and what is smaller to within 2^-18 of it; the tensor core sums them
+// to within 6e-8 of the sum of magnitudes.  Values go in as half-precision numbers, 16 of their elements on the side of
+// 16, so an output comes out transposed too.  One sequence of 32768 keys, 32 heads on 8: 25.9 us, where 16 rows a
+// product took 28.1; eight of 2048: 16.0 and 17.8.
+struct RowQueries {
+  unsigned b[2][D / 16];             // [part][four codes]
+  float factor[2];                   // of rows 2t, 2t + 1: what a product is multiplied by to be a score in log2 units
+  __device__ __forceinline__ void load(const Kv8Attention& p, const Entry& e, int kvh, int rows, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float x[D / 4];
+    unsigned big = 0u;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+    if (g < rows) {
+      const int token = g / p.groups, head = g - token * p.groups;
+      const bf16* src = p.q + (size_t)(e.tok0 + token) * p.q_stride + (size_t)(kvh * p.groups + head) * D;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) load4(src + Queries::element(s, t), x + 4 * s);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const bool finite = big < 0x7f800000u;
+    const int ex = finite ? kv8_exponent(big) : 0;
+    const float down = __int_as_float((127 - ex) << 23);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      unsigned word[2] = {0u, 0u};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const __half2 v = __floats2half2_rn(x[4 * s + 2 * k] * down, x[4 * s + 2 * k + 1] * down);
+        const unsigned hi = kv8_codes_of_half2(v), back = kv8_half2((unsigned short)hi);
+        word[0] |= hi << (16 * k);
+        word[1] |= kv8_codes_of_half2(__hsub2(v, *reinterpret_cast<const __half2*>(&back))) << (16 * k);
+      }
+      b[0][s] = word[0];
+      b[1][s] = word[1];
+    }
+    const float up = finite ? p.scale_log2 * __int_as_float((127 + ex) << 23) : kv8_scale(KV8_NAN);
+    factor[0] = __shfl_sync(0xffffffffu, up, 8 * t);             // row 2t lies with lanes 4 * 2t ..
+    factor[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+  }
+};
+
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// A fragment of 8 x 8 half-precision numbers, transposed
+__device__ __forceinline__ unsigned transposed(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+struct RowSums {
+  float m[2], l[2];                  // rows 2t, 2t + 1; l: of this lane's keys
+  float o[D / 16][4];                // m-tile i: elements (first, row 2t), (first, row 2t + 1), (second, ..), (second, ..)
+};
+
+// Value elements [BASE, BASE + 8 W): m-tile BASE/16 + 2c + h holds elements W g + 4 c + 2 h and the next one.
+template <int BASE, int W>
+__device__ __forceinline__ void row_values(const unsigned char* vs, int k0, const unsigned (&b)[2], RowSums& s, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  unsigned w[4][W / 4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = k0 + 2 * t + (i & 1) + 8 * (i >> 1), byte = BASE + W * g;
+    const typename Piece<W>::type x = *reinterpret_cast<const typename Piece<W>::type*>(vs + row * D + value_piece(row, byte >> 4) * 16 + (byte & 15));
+    if constexpr (W == 16) { w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w; }
+    else if constexpr (W == 8) { w[i][0] = x.x; w[i][1] = x.y; }
+    else w[i][0] = x;
+  }
+#pragma unroll
+  for (int c = 0; c < W / 4; ++c) {
+    unsigned a[2][4];
+    kv8_halves(__byte_perm(w[0][c], w[1][c], 0x5140), a[0][0], a[0][1]);
+    kv8_halves(__byte_perm(w[2][c], w[3][c], 0x5140), a[0][2], a[0][3]);
+    kv8_halves(__byte_perm(w[0][c], w[1][c], 0x7362), a[1][0], a[1][1]);
+    kv8_halves(__byte_perm(w[2][c], w[3][c], 0x7362), a[1][2], a[1][3]);
+    mma_f16(s.o[BASE / 16 + 2 * c], a[0], b[0], b[1]);
+    mma_f16(s.o[BASE / 16 + 2 * c + 1], a[1], b[0], b[1]);
+  }
+}
+
+// The 32 keys of a stage against eight rows.
+__device__ __forceinline__ void take_rows(const RowQueries& q, const unsigned char* stage, int key0, const Kv8Attention& p, bool clear,
+                                          const int (&pos)[2], RowSums& s, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  const float4* of_key = reinterpret_cast<const float4*>(stage + 2 * MATRIX);
+  float u[2][4];                     // [16 keys][(g, 2t), (g, 2t + 1), (g + 8, ..), (g + 8, ..)]
+  float back[2][2], mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    unsigned w[2][D / 16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 16 * j + 8 * h + g;
+#pragma unroll
+      for (int b = 0; b < D / 64; ++b) {
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + row * D + key_piece(row, 4 * b + t) * 16);
+        w[h][4 * b] = x.x; w[h][4 * b + 1] = x.y; w[h][4 * b + 2] = x.z; w[h][4 * b + 3] = x.w;
+      }
+      if constexpr ((D & 32) != 0) {
+        const uint2 x = *reinterpret_cast<const uint2*>(stage + row * D + D / 64 * 64 + 8 * t);
+        w[h][D / 64 * 4] = x.x; w[h][D / 64 * 4 + 1] = x.y;
+      }
+    }
+    float c[2][4];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) c[part][0] = c[part][1] = c[part][2] = c[part][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const unsigned a[4] = {w[0][2 * k], w[1][2 * k], w[0][2 * k + 1], w[1][2 * k + 1]};
+#pragma unroll
+      for (int part = 0; part < 2; ++part) mma_e4m3(c[part], a, q.b[part][2 * k], q.b[part][2 * k + 1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 of = of_key[16 * j + 8 * h + g];
+      back[j][h] = of.z;
+      const int key = key0 + 16 * j + 8 * h + g;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = fmaf((c[0][2 * h + i] + c[1][2 * h + i]) * of.x, q.factor[i], of.y);
+        if (!clear) {
+          const bool seen = key <= pos[i] && (p.window <= 0 || pos[i] - key < p.window || key < p.keep_first);
+          if (!seen) x = -INFINITY;
+        }
+        u[j][2 * h + i] = x;
+        mx[i] = fmaxf(mx[i], x);
+      }
+    }
+  }
+  float corr[2], base[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+    const float now = fmaxf(s.m[i], mx[i]);
+    corr[i] = s.m[i] == -INFINITY ? 0.f : exp2f(s.m[i] - now);
+    s.m[i] = now;
+    base[i] = now == -INFINITY ? 0.f : now;
+  }
+  if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+    s.l[0] *= corr[0];
+    s.l[1] *= corr[1];
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) { s.o[d][0] *= corr[0]; s.o[d][1] *= corr[1]; s.o[d][2] *= corr[0]; s.o[d][3] *= corr[1]; }
+  }
+  const unsigned char* vs = stage + MATRIX;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    unsigned b[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float w0 = exp2_fast(u[j][2 * h] - base[0]), w1 = exp2_fast(u[j][2 * h + 1] - base[1]);
+      s.l[0] = fmaf(w0, back[j][h], s.l[0]);
+      s.l[1] = fmaf(w1, back[j][h], s.l[1]);
+      b[h] = transposed(pack_half(w0, w1));
+    }
+    row_values<0, D >= 128 ? 16 : D >= 64 ? 8 : 4>(vs, 16 * j, b, s, lane);
+    if constexpr (D == 256) row_values<128, 16>(vs, 16 * j, b, s, lane);
+    if constexpr (D > 128 && D < 256 && (D & 64) != 0) row_values<128, 8>(vs, 16 * j, b, s, lane);
+    if constexpr (D > 64 && (D & 32) != 0) row_values<D / 64 * 64, 4>(vs, 16 * j, b, s, lane);
+  }
+}
+
+// First element of m-tile i (even i: four neighbouring ones, of m-tiles i and i + 1) for lane g.
+__device__ __forceinline__ int row_element(int i, int g) {
+  const int e0 = i * 16;
+  if (e0 < D / 128 * 128) return e0 / 128 * 128 + 16 * g + (i % 8) * 2;
+  int base = D / 128 * 128;
+  if ((D - base) & 64) {
+    if (e0 < base + 64) return base + 8 * g + (e0 - base) / 16 * 2;
+    base += 64;
+  }
+  return base + 4 * g + (e0 - base) / 16 * 2;
+}
+
+// What the warps of a block (their maxima, sums and value sums in `acc` and `ml`) make of its rows: the output, or a piece.
+__device__ __forceinline__ void finish_rows(const Kv8Attention& p, const Entry& e, int kvh, int n_rows, int pieces, const float* acc,
+                                            const float* ml, float* ws) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n_rows * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    float big = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) big = fmaxf(big, ml[(w * ROWS + r) * 2]);
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = piece_share(ml[(w * ROWS + r) * 2], ml[(w * ROWS + r) * 2 + 1], big);
+      const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROWS + r) * D + d);
+      num.x += x.x * f; num.y += x.y * f; num.z += x.z * f; num.w += x.w * f;
+      den += ml[(w * ROWS + r) * 2 + 1] * f;
+    }
+    if (pieces == 1) {
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      const float out[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+      const int token = r / p.groups, gq = r - token * p.groups;
+      store4(p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + gq) * D + d, out);
+    } else {
+      *reinterpret_cast<float4*>(ws + piece_element<ROWS>(r, d)) = num;
+      if (d == 0) { ws[(size_t)ROWS * D + 2 * r] = big; ws[(size_t)ROWS * D + 2 * r + 1] = den; }
+    }
+  }
+}
+
+// grid: (spans, entries, kv heads); a block takes `span` key tiles of an entry, warp w the keys 32 w .. 32 w + 31 of each.
+// Registers: for heads of up to 128, what three blocks an SM leave (their rings do not leave room for more).
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kernel(Kv8Attention p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_trigger();
+  pdl_wait();
+  const int entry = blockIdx.y, kvh = blockIdx.z, piece = blockIdx.x;
+  const Entry e(p, entry);
+  const int rows = e.n_new * p.groups;
+  if (rows <= p.row_lo || rows > p.row_hi) return;
+  const Walk<KEYS> walk(p, e.start, 0, rows);
+  const int pieces = pieces_of(p, walk.count);
+  if (piece >= pieces) return;
+  const int begin = piece * p.span, end = piece == pieces - 1 ? walk.count : begin + p.span, steps = end - begin;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  auto key0_of = [&](int i) -> int { return walk.tile(begin + i) * KEYS + warp * STEP; };
+  WarpRing mine(smem + warp * (STAGES * STAGE), p, p.block_table + (size_t)entry * p.max_pages, kvh, walk.key_lo, walk.key_end, lane);
+  mine.look_up(key0_of(0));
+  RowQueries q;
+  RowSums s;
+  int pos[2];                        // rows past the end take the last row's position; nobody reads them
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    pos[i] = e.start + min(2 * t + i, rows - 1) / p.groups;
+    s.m[i] = -INFINITY;
+    s.l[i] = 0.f;
+  }
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) { s.o[d][0] = s.o[d][1] = s.o[d][2] = s.o[d][3] = 0.f; }
+#pragma unroll 1
+  for (int i = -1; i < steps; ++i) {
+    if (i >= 0) mine.put_scales(i);
+    if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
+    cp_async_commit();
+    if (i < 0) {
+      q.load(p, e, kvh, rows, lane);
+      continue;
+    }
+    cp_async_wait<1>();
+    __syncwarp();
+    const int key0 = key0_of(i);
+    if (key0 <= walk.pos_last) {
+      const bool clear = key0 + STEP - 1 <= walk.pos_first && (p.window <= 0 || walk.pos_last - key0 < p.window);
+      take_rows(q, mine.stage(i), key0, p, clear, pos, s, lane);
+    }
+    __syncwarp();
+  }
+  __syncthreads();                   // the rings' space takes the warps' sums
+  float* acc = reinterpret_cast<float*>(smem);           // [WARPS][16][D]
+  float* ml = acc + WARPS * ROWS * D;                    // [WARPS][16][2]
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) s.l[i] += __shfl_xor_sync(0xffffffffu, s.l[i], o);
+    const int r = 2 * t + i;
+    if (r >= rows) continue;
+    float* to = acc + (warp * ROWS + r) * D;
+#pragma unroll
+    for (int d = 0; d < D / 16; d += 2)
+      *reinterpret_cast<float4*>(to + row_element(d, g)) = make_float4(s.o[d][i], s.o[d][2 + i], s.o[d + 1][i], s.o[d + 1][2 + i]);
+    if (g == 0) {
+      ml[(warp * ROWS + r) * 2] = s.m[i];
+      ml[(warp * ROWS + r) * 2 + 1] = s.l[i];
+    }
+  }
+  __syncthreads();
+  finish_rows(p, e, kvh, rows, pieces, acc, ml, p.ws + (((size_t)entry * p.nkv + kvh) * p.spans + piece) * ROWS * (D + 2));
+}
+
+// ---- 9 to 16 rows, any number of head sizes that are no whole 32s, portions of head sizes other than 64 and 128 ----
+//
 // PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of its tiles.  Otherwise it takes the (at most
 // 16) rows of an entry, and warp w the keys 32 w .. 32 w + 31 of every tile; the warps' sums join at the end.
-// A warp goes its own way: it copies its keys into a ring of its own, a step ahead, and waits for nobody (with a ring of the
-// block and a barrier a tile, 64 keys of one head took 1.7 us a block whatever else ran).  A lane looks after one key: its
-// page, two steps ahead, its place and its scales.
 // grid: (spans, row tiles - single tokens: entries -, kv heads); a block takes `span` key tiles of its unit.
 template <bool PORTION>
 __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
@@ -337,8 +659,6 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   auto key0_of = [&](int i) -> int {
     return PORTION ? walk.tile(begin + i / (KEYS / STEP)) * KEYS + i % (KEYS / STEP) * STEP : walk.tile(begin + i) * KEYS + warp * STEP;
   };
-  auto look_up = [&](int i) -> int { return i < steps ? key_page(p, table, key0_of(i) + lane, walk.key_end) : -1; };
-
   const int wrow0 = PORTION ? row0 + warp * ROWS : row0;
   // rows past the end take the last row's position; nobody reads them
   const int last = rows_end - 1;
@@ -347,34 +667,12 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   Queries q;
   Sums s;
   s.clear();
-  int page = look_up(0);
-  int k_scale = KV8_BIAS, v_scale = KV8_BIAS;       // of this lane's key of the step whose copies were asked for last
+  WarpRing mine(ring, p, table, kvh, walk.key_lo, walk.key_end, lane);
+  mine.look_up(key0_of(0));
 #pragma unroll 1
   for (int i = -1; i < steps; ++i) {
-    if (i >= 0) {
-      // the scales of step i, asked for with its copies; a key whose value is not finite counts as not finite itself
-      float* of_key = reinterpret_cast<float*>(ring + (i & 1) * STAGE + 2 * MATRIX);
-      const bool bad = v_scale == KV8_NAN;
-      of_key[lane] = kv8_scale(bad ? KV8_NAN : k_scale);
-      of_key[STEP + lane] = bad ? 0.f : (float)(v_scale - KV8_BIAS);
-      of_key[2 * STEP + lane] = bad ? 1.f : __int_as_float((2 * KV8_BIAS - v_scale) << 23);
-    }
-    if (i + 1 < steps) {
-      const int key = key0_of(i + 1) + lane;
-      long long at;
-      const bool there = key_row(p, page, kvh, key, &at);
-      if (!there) tell_missing(p, key, walk.key_lo, walk.key_end);
-      k_scale = v_scale = KV8_BIAS;
-      if (there) {
-        k_scale = __ldg(p.ks + at);
-        v_scale = __ldg(p.vs + at);
-      }
-      page = look_up(i + 2);
-      const int mine = there ? (int)at : -1;             // the launcher holds the rows of a cache to 31 bits
-      unsigned char* stage = ring + ((i + 1) & 1) * STAGE;
-      if (__all_sync(0xffffffffu, there)) copy_step<true>(p, stage, mine, lane);
-      else copy_step<false>(p, stage, mine, lane);
-    }
+    if (i >= 0) mine.put_scales(i);
+    if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
     cp_async_commit();
     if (i < 0) {
       q.load(p, e, kvh, wrow0, rows_end, lane);
@@ -440,48 +738,39 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
       }
     }
     __syncthreads();
-#pragma unroll 1
-    for (int i = threadIdx.x; i < n_rows * (D / 4); i += THREADS) {
-      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-      float big = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) big = fmaxf(big, ml[(w * ROWS + r) * 2]);
-      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-      float den = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = piece_share(ml[(w * ROWS + r) * 2], ml[(w * ROWS + r) * 2 + 1], big);
-        const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROWS + r) * D + d);
-        num.x += x.x * f; num.y += x.y * f; num.z += x.z * f; num.w += x.w * f;
-        den += ml[(w * ROWS + r) * 2 + 1] * f;
-      }
-      if (pieces == 1) {
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-        const float out[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
-        const int row = row0 + r, token = row / p.groups, gq = row - token * p.groups;
-        store4(p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + gq) * D + d, out);
-      } else {
-        *reinterpret_cast<float4*>(ws + piece_element<UNIT>(r, d)) = num;
-        if (d == 0) { ws[(size_t)UNIT * D + 2 * r] = big; ws[(size_t)UNIT * D + 2 * r + 1] = den; }
-      }
-    }
+    finish_rows(p, e, kvh, n_rows, pieces, acc, ml, ws);
   }
 }
 
-template <bool PORTION>
-int launch_mma(Kv8Attention p, cudaStream_t stream) {
-  constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
-  const long long slots = PORTION ? portion_slots(p.entries, p.total_tokens, p.groups, UNIT) : p.entries;
+template <typename Kernel>
+int launch_blocks(Kernel kernel, const Kv8Attention& p, cudaStream_t stream) {
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM);
+  if (err != cudaSuccess) return (int)err;
+  return fe_launch_dependent(kernel, dim3((unsigned)p.spans, (unsigned)p.slots, (unsigned)p.nkv), dim3(THREADS), MMA_SMEM, stream, p);
+}
+
+// Entries with row_lo < rows <= row_hi, at most 16.
+int launch_single(Kv8Attention p, cudaStream_t stream) {
+  p.slots = p.entries;
+  int rc = 0;
+#if FE_HEAD_DIM % 32 == 0
+  rc = p.row_hi <= 8 ? launch_blocks(attn_kv8_rows_kernel, p, stream) : launch_blocks(attn_kv8_mma_kernel<false>, p, stream);
+#else
+  rc = launch_blocks(attn_kv8_mma_kernel<false>, p, stream);
+#endif
+  return rc || p.spans == 1 ? rc : launch_join<ROWS, KEYS, false>(p, stream);
+}
+
+#if FE_HEAD_DIM != 64 && FE_HEAD_DIM != 128
+int launch_portion(Kv8Attention p, cudaStream_t stream) {
+  constexpr int UNIT = ROWS * WARPS;
+  const long long slots = portion_slots(p.entries, p.total_tokens, p.groups, UNIT);
   if (slots > 65535) return FE_ERR_TOO_LARGE;
   p.slots = (int)slots;
-  const cudaError_t err = cudaFuncSetAttribute(attn_kv8_mma_kernel<PORTION>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM);
-  if (err != cudaSuccess) return (int)err;
-  int rc = fe_launch_dependent(attn_kv8_mma_kernel<PORTION>, dim3((unsigned)p.spans, (unsigned)p.slots, (unsigned)p.nkv), dim3(THREADS), MMA_SMEM,
-                               stream, p);
-  if (rc == 0 && p.spans > 1)
-    rc = launch_join<UNIT, KEYS, PORTION>(p, stream);
-  return rc;
+  const int rc = launch_blocks(attn_kv8_mma_kernel<true>, p, stream);
+  return rc || p.spans == 1 ? rc : launch_join<UNIT, KEYS, true>(p, stream);
 }
+#endif
 
 }  // namespace
 
@@ -497,18 +786,18 @@ FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, 
   return slots * nkv * spans * unit * (D + 2);
 }
 
-// The entries of a step with at most 16 rows (new tokens x heads per kv head) if single_spans is above zero, the others
-// if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
+// The entries of a step with at most 8 rows (new tokens x heads per kv head) if few_spans is above zero, those with 9 to 16
+// if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
                                       int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int total_tokens,
-                                      int window, int keep_first, float scale, int single_span,
-                                      int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
+                                      int window, int keep_first, float scale, int few_span, int few_spans,
+                                      int single_span, int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
                                       cudaStream_t stream) {
   if (entries <= 0 || total_tokens <= 0) return 0;
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
-  if (single_spans < 0 || portion_spans < 0 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
-  if ((single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
+  if (few_spans < 0 || single_spans < 0 || portion_spans < 0 || few_span < 1 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
+  if ((few_spans > 1 || single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
   if ((long long)num_pages * nkv > 0x7fffffffLL / page_size) return FE_ERR_TOO_LARGE;       // rows of a cache: 31 bits
   if (entries > 65535 || nkv > 65535 || (long long)total_tokens * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
   if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) ||
@@ -525,18 +814,19 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   p.entries = entries; p.slots = 0;
   p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.ws = workspace;
+  if (few_spans > 0) {
+    p.row_lo = 0; p.row_hi = 8; p.span = few_span; p.spans = few_spans;
+    const int rc = launch_single(p, stream);
+    if (rc) return rc;
+  }
   if (single_spans > 0) {
-    p.row_lo = 0; p.row_hi = ROWS; p.span = single_span; p.spans = single_spans;
-    const int rc = launch_mma<false>(p, stream);
+    p.row_lo = 8; p.row_hi = ROWS; p.span = single_span; p.spans = single_spans;
+    const int rc = launch_single(p, stream);
     if (rc) return rc;
   }
   if (portion_spans > 0) {
     p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans;
-#if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
     const int rc = launch_portion(p, stream);
-#else
-    const int rc = launch_mma<true>(p, stream);
-#endif
     if (rc) return rc;
   }
   return fe_last_error();

@@ -1890,7 +1890,7 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor, status: torch.Tensor, w
 # ---------------------------------------------------------------------------
 
 KV8_CODES, KV8_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
-KV8_SINGLE_ROWS = 16         # rows (new tokens x heads per kv head) of an entry that the kernel of single tokens takes
+KV8_FEW_ROWS, KV8_SINGLE_ROWS = 8, 16     # rows (new tokens x heads per kv head) of an entry that the kernels of single tokens take
 KV8_TILE = 128               # keys of a tile
 KV8_TC5_DIMS = (64, 128)     # head sizes whose portions the tcgen05 kernel takes
 
@@ -1913,7 +1913,7 @@ def kv8_lib(head_dim: int):
             raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
         p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
         fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
-        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, f, i, i, i, i, p, p, p]
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, f, i, i, i, i, i, i, p, p, p]
         fn.restype = c_int
         size.argtypes = [i, i, i, i, i, i]
         size.restype = ll
@@ -2054,9 +2054,9 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
 
 
 def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window: int | None = None, keep_first: int = 0) -> tuple:
-    """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries (tuples): (key tiles a
-    block takes of an entry with at most 16 rows, such blocks of the longest one, and both for the other entries);
-    a count of 0: there is no such entry.  Layers of one geometry share it."""
+    """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries (tuples): the key tiles a
+    block takes of an entry and such blocks of the longest one, for entries with at most 8 rows (new tokens x heads per kv
+    head), with 9 to 16, and the others; 0 blocks: there is no such entry.  Layers of one geometry share it."""
     return _kv8_plan(tuple(entries), num_q_heads // num_kv_heads, num_kv_heads, head_dim, window or 0, keep_first or 0)
 
 
@@ -2083,15 +2083,15 @@ _KV8_SPANS = tuple(sorted({m << e for e in range(0, 22) for m in (2, 3)} | {1}))
 def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int, keep_first: int) -> tuple:
     tc5 = head_dim in KV8_TC5_DIMS
     rows_of = 256 if tc5 else 64
-    single, portion = [], []
+    few, single, portion = [], [], []
     for start, count in entries:
         rows = count * groups
         if 0 < rows <= KV8_SINGLE_ROWS:
-            single.append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
+            (few if rows <= KV8_FEW_ROWS else single).append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
         elif rows:
             for row in range(0, rows, rows_of):
                 portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
-    return (*_kv8_cut(single, nkv, *_KV8_SINGLE), *_kv8_cut(portion, nkv, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
+    return (*_kv8_cut(few, nkv, *_KV8_SINGLE), *_kv8_cut(single, nkv, *_KV8_SINGLE), *_kv8_cut(portion, nkv, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
 
 
 def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block: float, join: float, piece: float) -> tuple:
@@ -2147,18 +2147,18 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             or block_table.shape[0] < n_entries):
         raise UnsupportedShapeError("cu_tokens holds entries + 1 int32 numbers, starts one an entry, block_table a row")
     index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out), (q,))
-    single_span, single_spans, portion_span, portion_spans = plan
+    few_span, few_spans, single_span, single_spans, portion_span, portion_spans = plan
     groups = num_q_heads // nkv
     if max_new * groups <= KV8_SINGLE_ROWS:
         portion_spans = 0
     fn, size = kv8_lib(d)
     workspace = None
-    if single_spans > 1 or portion_spans > 1:
+    if few_spans > 1 or single_spans > 1 or portion_spans > 1:
         # the pieces of a cut entry meet in a buffer of the call's own: calls on other streams, and captured ones, have theirs
-        numbers = max(size(0, n_entries, nkv, groups, n, single_spans), size(1, n_entries, nkv, groups, n, portion_spans))
+        numbers = max(size(0, n_entries, nkv, groups, n, max(few_spans, single_spans)), size(1, n_entries, nkv, groups, n, portion_spans))
         workspace = torch.empty(numbers, dtype=torch.float32, device=q.device)
     _kv8_call(index, fn,
               (q.data_ptr(), q_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                block_table.data_ptr(), block_table.shape[1], page_size, num_pages, nkv, groups, cu_tokens.data_ptr(),
-               starts.data_ptr(), n_entries, n, window, keep_first, scale, single_span, single_spans, portion_span,
+               starts.data_ptr(), n_entries, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_span,
                portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")

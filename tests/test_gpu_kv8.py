@@ -260,7 +260,7 @@ def test_attention(native, dim, heads, nkv, page, requests, window, keep) -> Non
     check_attention(cache, requests, q, out, window, keep, scale)
 
 
-@pytest.mark.parametrize("dim,requests", [(128, [(900, 1), (333, 1), (10, 1)]), (64, [(700, 200), (90, 40)]), (128, [(700, 200), (90, 40), (64, 1)]),
+@pytest.mark.parametrize("dim,requests", [(128, [(900, 1), (333, 1), (10, 1)]), (128, [(700, 3), (90, 4), (64, 1)]), (48, [(300, 1), (200, 4)]), (96, [(300, 2), (200, 3)]), (64, [(700, 200), (90, 40)]), (128, [(700, 200), (90, 40), (64, 1)]),
                                           (32, [(700, 90)])])
 def test_attention_cut_into_pieces(native, dim, requests) -> None:
     """Every cut of the keys gives the same attention; a plan made for shorter entries still sees all keys."""
@@ -268,7 +268,7 @@ def test_attention_cut_into_pieces(native, dim, requests) -> None:
     cache = plain.pool([s + n for s, n in requests], nkv, dim, page, dim)
     g = torch.Generator().manual_seed(4)
     q = (torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=g) * 2).to(torch.bfloat16)
-    for spans in ((1, 16, 1, 16), (2, 8, 3, 8), (3, 4, 2, 2), (1, 2, 1, 2), (100, 1, 100, 1)):
+    for spans in ((1, 16, 1, 16, 1, 16), (2, 8, 2, 8, 3, 8), (3, 4, 3, 4, 2, 2), (1, 2, 1, 2, 1, 2), (100, 1, 100, 1, 100, 1)):
         for window, keep in ((0, 0), (200, 20)):
             out, status = attend(native, cache, requests, q, window, keep, dim ** -0.5, plan=spans)
             assert status == 0
@@ -351,7 +351,7 @@ def test_bad_token_counts_touch_nothing(native) -> None:
     caches = to_device(cache)
     q = torch.randn((4, heads * dim)).to(torch.bfloat16).to(DEV)
     for ends, starts in (([0, 5, 6], [0, 0]), ([-1, 2, 3], [0, 0]), ([3, 1, 1], [0, 0]), ([0, 1, 2], [-5, -1])):
-        for plan in ((1, 2, 1, 2), (4, 1, 4, 1)):
+        for plan in ((1, 2, 1, 2, 1, 2), (4, 1, 4, 1, 4, 1)):
             out, status = torch.full_like(q, 7.0), status_word()
             native.attention_kv8(q, *caches, cache["table"].to(DEV), ints(ends), ints(starts), 1, 5, heads, 0, 0, 1.0, out, status, plan)
             assert int(status.item()) == 4 and bool((out == 7.0).all())
@@ -410,7 +410,7 @@ def test_two_captured_graphs_and_eager_calls_between(native) -> None:
         args = (q.to(DEV), *to_device(cache), cache["table"].to(DEV), ints(ends), ints(s for s, _ in requests), len(requests),
                 max(n for _, n in requests), heads, 0, 0, dim ** -0.5)
         cases.append((cache, requests, q, args, torch.zeros(q.shape, dtype=torch.bfloat16, device=DEV), status_word()))
-    plan = (2, 8, 2, 8)
+    plan = (2, 8, 2, 8, 2, 8)
     graphs, streams = [], []
     for cache, requests, q, args, out, status in cases:
         native.attention_kv8(*args, out, status, plan)

@@ -35,7 +35,7 @@ def attention_args(**other):
     args = {**caches(), "q": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "block_table": torch.zeros((2, 3), dtype=torch.int32),
             "cu_tokens": torch.tensor([0, 1, 6], dtype=torch.int32), "starts": torch.zeros(2, dtype=torch.int32), "n_entries": 2,
             "max_new": 5, "num_q_heads": HEADS, "window": None, "keep_first": 0, "scale": 1.0,
-            "out": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "status": torch.zeros(1, dtype=torch.int32), "plan": (1, 1, 1, 1)}
+            "out": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "status": torch.zeros(1, dtype=torch.int32), "plan": (1, 1, 1, 1, 1, 1)}
     return {**args, **other}
 
 
@@ -116,11 +116,11 @@ def test_quantising_restates_the_type() -> None:
 @pytest.mark.parametrize("entries", [[(0, 1)], [(5000, 1), (0, 1), (300, 2)], [(0, 2048)], [(32768, 1)], [(10, 0), (4000, 700), (9, 1)], [(7, 0)], []])
 def test_plans_cover_every_key(entries, window, keep) -> None:
     for heads, nkv, dim in ((32, 8, 128), (4, 4, 64), (16, 1, 96)):
-        single_span, single_spans, portion_span, portion_spans = native.kv8_plan(entries, heads, nkv, dim, window, keep)
+        plan = native.kv8_plan(entries, heads, nkv, dim, window, keep)
         groups = heads // nkv
-        rows = [n * groups for _, n in entries]
-        assert (single_spans > 0) == any(0 < r <= 16 for r in rows) and (portion_spans > 0) == any(r > 16 for r in rows)
-        for (start, n), r in zip(entries, rows):
-            if r and not window:
-                span, spans = (single_span, single_spans) if r <= 16 else (portion_span, portion_spans)
-                assert span >= 1 and spans >= 1 and (spans & (spans - 1)) == 0 and span * spans * native.KV8_TILE >= start + n
+        kinds = [(lambda r: 0 < r <= 8, plan[:2]), (lambda r: 8 < r <= 16, plan[2:4]), (lambda r: r > 16, plan[4:])]
+        for is_kind, (span, spans) in kinds:
+            mine = [start + n for start, n in entries if is_kind(n * groups)]
+            assert (spans > 0) == bool(mine) and span >= 1 and (spans & (spans - 1)) == 0
+            if mine and not window:
+                assert span * spans * native.KV8_TILE >= max(mine)
