@@ -557,13 +557,15 @@ __device__ __forceinline__ void finish_rows(const Kv8Attention& p, const Entry& 
   }
 }
 
-// grid: (spans, entries, kv heads); a block takes `span` key tiles of an entry, warp w the keys 32 w .. 32 w + 31 of each.
+// grid: (kv heads, entries, spans); a block takes `span` key tiles of an entry, warp w the keys 32 w .. 32 w + 31 of each.
+// Blocks past an entry's last piece come last: in between they left the SMs unevenly filled (32768 keys: 25.2 us with 40
+// spans of which 33 have keys).
 // Registers: for heads of up to 128, what three blocks an SM leave (their rings do not leave room for more).
 __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kernel(Kv8Attention p) {
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_trigger();
   pdl_wait();
-  const int entry = blockIdx.y, kvh = blockIdx.z, piece = blockIdx.x;
+  const int kvh = blockIdx.x, entry = blockIdx.y, piece = blockIdx.z;
   const Entry e(p, entry);
   const int rows = e.n_new * p.groups;
   if (rows <= p.row_lo || rows > p.row_hi) return;
@@ -630,14 +632,15 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kerne
 //
 // PORTION: a block takes 64 rows, 16 a warp, and every warp all keys of its tiles.  Otherwise it takes the (at most
 // 16) rows of an entry, and warp w the keys 32 w .. 32 w + 31 of every tile; the warps' sums join at the end.
-// grid: (spans, row tiles - single tokens: entries -, kv heads); a block takes `span` key tiles of its unit.
+// grid: (kv heads, row tiles - single tokens: entries -, spans); a block takes `span` key tiles of its unit, the row tiles
+// that see most keys first.
 template <bool PORTION>
 __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
   pdl_trigger();
   pdl_wait();
-  const int slot = blockIdx.y, kvh = blockIdx.z, piece = blockIdx.x;
+  const int kvh = blockIdx.x, slot = PORTION ? gridDim.y - 1 - blockIdx.y : blockIdx.y, piece = blockIdx.z;
   int entry = slot, unit = 0;
   if constexpr (PORTION) {
     const Slot<UNIT> at(p, slot);
@@ -746,7 +749,14 @@ template <typename Kernel>
 int launch_blocks(Kernel kernel, const Kv8Attention& p, cudaStream_t stream) {
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM);
   if (err != cudaSuccess) return (int)err;
-  return fe_launch_dependent(kernel, dim3((unsigned)p.spans, (unsigned)p.slots, (unsigned)p.nkv), dim3(THREADS), MMA_SMEM, stream, p);
+  if (p.spans > 65535) return FE_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)p.nkv, (unsigned)p.slots, (unsigned)p.spans);
+  if (p.spans == 1) return fe_launch_dependent(kernel, grid, dim3(THREADS), MMA_SMEM, stream, p);
+  // Cut entries fill the SMs by count, so no block of theirs is to be placed while the kernel before still holds some of
+  // them: as a dependent launch one token behind 32768 keys takes 21.3 to 25.2 us from one count of spans to the next,
+  // without 21.4 for all (48 uncut windows of 15 rows behind a cache write: 85.7 as a dependent launch, 87.3 without).
+  kernel<<<grid, THREADS, MMA_SMEM, stream>>>(p);
+  return (int)cudaGetLastError();
 }
 
 // Entries with row_lo < rows <= row_hi, at most 16.
@@ -758,7 +768,7 @@ int launch_single(Kv8Attention p, cudaStream_t stream) {
 #else
   rc = launch_blocks(attn_kv8_mma_kernel<false>, p, stream);
 #endif
-  return rc || p.spans == 1 ? rc : launch_join<ROWS, KEYS, false>(p, stream);
+  return rc || p.spans == 1 ? rc : launch_join<ROWS, KEYS>(p, stream);
 }
 
 #if FE_HEAD_DIM != 64 && FE_HEAD_DIM != 128
@@ -768,7 +778,7 @@ int launch_portion(Kv8Attention p, cudaStream_t stream) {
   if (slots > 65535) return FE_ERR_TOO_LARGE;
   p.slots = (int)slots;
   const int rc = launch_blocks(attn_kv8_mma_kernel<true>, p, stream);
-  return rc || p.spans == 1 ? rc : launch_join<UNIT, KEYS, true>(p, stream);
+  return rc || p.spans == 1 ? rc : launch_join_portion<UNIT, KEYS>(p, stream);
 }
 #endif
 
@@ -790,11 +800,11 @@ FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, 
 // if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
-                                      int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int total_tokens,
+                                      int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new, int total_tokens,
                                       int window, int keep_first, float scale, int few_span, int few_spans,
                                       int single_span, int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
                                       cudaStream_t stream) {
-  if (entries <= 0 || total_tokens <= 0) return 0;
+  if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
   if (few_spans < 0 || single_spans < 0 || portion_spans < 0 || few_span < 1 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
   if ((few_spans > 1 || single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
@@ -811,7 +821,7 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   for (int s = 0; s < 31; ++s)
     if (page_size == 1 << s) p.page_shift = s;
   p.nkv = nkv; p.groups = groups; p.cu_tokens = cu_tokens; p.starts = starts; p.total_tokens = total_tokens;
-  p.entries = entries; p.slots = 0;
+  p.entries = entries; p.max_new = max_new; p.slots = 0;
   p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.ws = workspace;
   if (few_spans > 0) {

@@ -27,7 +27,7 @@ struct Kv8Attention {
   int* status;
   int row_lo, row_hi;      // entries with row_lo < rows <= row_hi
   int span, spans;         // a block takes `span` key tiles of a unit; the grid holds `spans` of them
-  int entries;
+  int entries, max_new;    // max_new: the most tokens an entry has
   int slots;               // row tiles of all entries, at most: see Slot
   float* ws;               // [slots, nkv, spans][rows of a unit x (D + 2)]: see piece_element
 };
@@ -59,7 +59,7 @@ struct Entry {
     tok0 = p.cu_tokens[entry];
     n_new = p.cu_tokens[entry + 1] - tok0;
     start = p.starts[entry];
-    if (tok0 < 0 || n_new < 0 || tok0 > p.total_tokens - n_new || start < 0 || start > 0x7fff0000 - n_new) {
+    if (tok0 < 0 || n_new < 0 || n_new > p.max_new || tok0 > p.total_tokens - n_new || start < 0 || start > 0x7fff0000 - n_new) {
       if (threadIdx.x == 0) atomicOr(p.status, FE_STATUS_BAD_POSITION);
       n_new = 0;
     }
@@ -127,40 +127,28 @@ inline long long portion_slots(int entries, int total_tokens, int groups, int un
   return (long long)total_tokens * groups / unit + entries;
 }
 
-// Joins the pieces of a unit's rows, in the order of the keys: a lane takes D / 32 (at least two) neighbouring columns
-// of a row and works out one piece's share of 32.  Portions have few pieces and many rows: four rows a block, a warp
-// each.  A single token's row may have a hundred pieces: a block a row, its eight warps every eighth piece, their sums
-// joined in the order of the warps (one warp a row: 13.8 us for 103 pieces).
-// grid: (rows of the slots / rows of a block, kv heads)
-template <bool PORTION> constexpr int JOIN_ROWS = PORTION ? 4 : 1;
-template <bool PORTION> constexpr int JOIN_WARPS = PORTION ? 4 : 8;
+// Joins the pieces of a single token's rows.  A row may have a hundred of them: a block a row, its eight warps every
+// eighth piece, a lane D / 32 (at least two) neighbouring columns and one piece's share of 32; the warps' sums are
+// joined in their order (one warp a row: 13.8 us for 103 pieces).  The grid holds no more rows than an entry can have.
+// grid: (entries * rows of an entry, kv heads)
+constexpr int JOIN_WARPS = 8;
 
-template <int UNIT, int TILE, bool PORTION>
-__global__ void __launch_bounds__(32 * JOIN_WARPS<PORTION>) attn_kv8_join_kernel(Kv8Attention p) {
+template <int UNIT, int TILE>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Attention p, int rows_most) {
   constexpr int COLUMNS = D >= 128 ? 4 : 2, LANES_D = 32 * COLUMNS;
   constexpr int PASSES = (D + LANES_D - 1) / LANES_D;
-  constexpr int BLOCKS = UNIT / JOIN_ROWS<PORTION>, SHARE = PORTION ? 1 : JOIN_WARPS<PORTION>;
-  __shared__ float sums[SHARE][PASSES * LANES_D], dens[SHARE];
+  __shared__ float sums[JOIN_WARPS][PASSES * LANES_D], dens[JOIN_WARPS];
   pdl_trigger();
   pdl_wait();
-  const int slot = blockIdx.x / BLOCKS, kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int entry = slot, unit = 0;
-  if constexpr (PORTION) {
-    const Slot<UNIT> at(p, slot);
-    entry = at.entry;
-    unit = at.unit;
-  }
+  const int entry = blockIdx.x / rows_most, kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Entry e(p, entry);
-  const int rows = e.n_new * p.groups, row0 = unit * UNIT;
-  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
-  const int rows_end = min(rows, row0 + UNIT);
-  const int r = (blockIdx.x - slot * BLOCKS) * JOIN_ROWS<PORTION> + (PORTION ? warp : 0);
-  if (row0 + r >= rows_end) return;
-  const Walk<TILE> walk(p, e.start, row0, rows_end);
+  const int rows = e.n_new * p.groups, r = blockIdx.x - entry * rows_most;
+  if (rows <= p.row_lo || rows > p.row_hi || r >= rows) return;
+  const Walk<TILE> walk(p, e.start, 0, rows);
   const int pieces = pieces_of(p, walk.count);
   if (pieces == 1) return;
   const size_t step = (size_t)UNIT * (D + 2);
-  const float* ws = p.ws + ((size_t)slot * p.nkv + kvh) * p.spans * step;
+  const float* ws = p.ws + ((size_t)entry * p.nkv + kvh) * p.spans * step;
   const float* ml = ws + (size_t)UNIT * D + 2 * r;
   float big = -INFINITY;
   for (int s = lane; s < pieces; s += 32) big = fmaxf(big, ml[s * step]);
@@ -170,11 +158,11 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS<PORTION>) attn_kv8_join_kernel
   for (int i = 0; i < PASSES; ++i)
 #pragma unroll
     for (int c = 0; c < COLUMNS; ++c) num[i][c] = 0.f;
-  const int first = PORTION ? 0 : warp, mine = (pieces - first + SHARE - 1) / SHARE;        // pieces first, first + SHARE, ...
+  const int mine = (pieces - warp + JOIN_WARPS - 1) / JOIN_WARPS;         // pieces warp, warp + 8, ...
   for (int k0 = 0; k0 < mine; k0 += 32) {
     float share = 0.f;
     if (k0 + lane < mine) {
-      const float* at = ml + (size_t)(first + (k0 + lane) * SHARE) * step;
+      const float* at = ml + (size_t)(warp + (k0 + lane) * JOIN_WARPS) * step;
       share = piece_share(at[0], at[1], big);
       den += at[1] * share;
     }
@@ -182,7 +170,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS<PORTION>) attn_kv8_join_kernel
 #pragma unroll 8
     for (int k = 0; k < here; ++k) {
       const float f = __shfl_sync(0xffffffffu, share, k);
-      const float* src = ws + (size_t)(first + (k0 + k) * SHARE) * step;
+      const float* src = ws + (size_t)(warp + (k0 + k) * JOIN_WARPS) * step;
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int d = i * LANES_D + lane * COLUMNS;
@@ -198,38 +186,99 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS<PORTION>) attn_kv8_join_kernel
     }
   }
   den = warp_sum(den);
-  if constexpr (!PORTION) {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i)
+  for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-      for (int c = 0; c < COLUMNS; ++c) sums[warp][i * LANES_D + lane * COLUMNS + c] = num[i][c];
-    if (lane == 0) dens[warp] = den;
-    __syncthreads();
-    den = 0.f;
+    for (int c = 0; c < COLUMNS; ++c) sums[warp][i * LANES_D + lane * COLUMNS + c] = num[i][c];
+  if (lane == 0) dens[warp] = den;
+  __syncthreads();
+  den = 0.f;
 #pragma unroll
-    for (int w = 0; w < SHARE; ++w) den += dens[w];
-    for (int d = threadIdx.x; d < D; d += 32 * SHARE) {
-      float x = 0.f;
+  for (int w = 0; w < JOIN_WARPS; ++w) den += dens[w];
+  for (int d = threadIdx.x; d < D; d += 32 * JOIN_WARPS) {
+    float x = 0.f;
 #pragma unroll
-      for (int w = 0; w < SHARE; ++w) x += sums[w][d];
-      store_row(p, e, kvh, row0 + r, d, den == 0.f ? 0.f : x / den);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int d = i * LANES_D + lane * COLUMNS;
-      if (D % LANES_D == 0 || d < D) {
-#pragma unroll
-        for (int c = 0; c < COLUMNS; ++c) store_row(p, e, kvh, row0 + r, d + c, den == 0.f ? 0.f : num[i][c] / den);
-      }
-    }
+    for (int w = 0; w < JOIN_WARPS; ++w) x += sums[w][d];
+    store_row(p, e, kvh, r, d, den == 0.f ? 0.f : x / den);
   }
 }
 
-template <int UNIT, int TILE, bool PORTION>
+// Joins the pieces of a portion's rows, in the order of the keys: a thread takes eight columns of a row, eight lanes eight
+// rows, so that a warp reads 256 bytes in a line and its stores fill 64.  Portions have few pieces and many rows.
+// grid: (slots * UNIT / rows of a block, kv heads)
+constexpr int JOIN_ROWS = D <= 64 ? 32 : D <= 128 ? 16 : 8;         // eight columns of a row a thread
+template <int UNIT, int TILE>
+__global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention p) {
+  constexpr int BLOCKS = UNIT / JOIN_ROWS, STRETCHES = D / 8, BATCH = 8;
+  pdl_trigger();
+  pdl_wait();
+  const int slot = blockIdx.x / BLOCKS, kvh = blockIdx.y;
+  const Slot<UNIT> at(p, slot);
+  const Entry e(p, at.entry);
+  const int rows = e.n_new * p.groups, row0 = at.unit * UNIT, r0 = (blockIdx.x - slot * BLOCKS) * JOIN_ROWS;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 + r0 >= rows) return;
+  const int rows_end = min(rows, row0 + UNIT);
+  const Walk<TILE> walk(p, e.start, row0, rows_end);
+  const int pieces = pieces_of(p, walk.count);
+  if (pieces == 1) return;
+  const size_t step = (size_t)UNIT * (D + 2);
+  const float* ws = p.ws + ((size_t)slot * p.nkv + kvh) * p.spans * step;
+  const int i = threadIdx.x, r = r0 + (i & 7) + 8 * (i / (8 * STRETCHES)), d = 8 * ((i >> 3) % STRETCHES);
+  if (i >= JOIN_ROWS * STRETCHES || row0 + r >= rows_end) return;
+  const float* ml = ws + (size_t)UNIT * D + 2 * r;
+  float big = -INFINITY, den = 0.f, num[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) num[c] = 0.f;
+  for (int s0 = 0; s0 < pieces; s0 += BATCH) {
+    float2 of[BATCH];
+    float4 a[BATCH], b[BATCH];
+    float now = big;
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      of[s] = make_float2(-INFINITY, 0.f);
+      a[s] = b[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + s < pieces) {
+        of[s] = *reinterpret_cast<const float2*>(ml + (s0 + s) * step);
+        const float4* src = reinterpret_cast<const float4*>(ws + (s0 + s) * step + piece_element<UNIT>(r, d));
+        a[s] = src[0];
+        b[s] = src[1];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) now = fmaxf(now, of[s].x);
+    const float corr = big == -INFINITY ? 1.f : exp2f(big - now);         // what is there without a maximum is 0 or NaN
+    den *= corr;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) num[c] *= corr;
+    big = now;
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      const float share = piece_share(of[s].x, of[s].y, big);
+      den += of[s].y * share;
+      num[0] += a[s].x * share; num[1] += a[s].y * share; num[2] += a[s].z * share; num[3] += a[s].w * share;
+      num[4] += b[s].x * share; num[5] += b[s].y * share; num[6] += b[s].z * share; num[7] += b[s].w * share;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 8; ++c) num[c] = den == 0.f ? 0.f : num[c] / den;
+  const int row = row0 + r, token = row / p.groups, g = row - token * p.groups;
+  bf16* to = p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D + d;
+  store4(to, num);
+  store4(to + 4, num + 4);
+}
+
+template <int UNIT, int TILE>
 inline int launch_join(const Kv8Attention& p, cudaStream_t stream) {
-  return fe_launch_dependent(attn_kv8_join_kernel<UNIT, TILE, PORTION>, dim3((unsigned)(p.slots * (UNIT / JOIN_ROWS<PORTION>)), (unsigned)p.nkv),
-                             dim3(32 * JOIN_WARPS<PORTION>), 0, stream, p);
+  const long long most = (long long)p.max_new * p.groups;
+  const int rows = most < p.row_hi ? (int)most : p.row_hi;
+  return fe_launch_dependent(attn_kv8_join_kernel<UNIT, TILE>, dim3((unsigned)(p.slots * rows), (unsigned)p.nkv), dim3(32 * JOIN_WARPS), 0,
+                             stream, p, rows);
+}
+
+template <int UNIT, int TILE>
+inline int launch_join_portion(const Kv8Attention& p, cudaStream_t stream) {
+  return fe_launch_dependent(attn_kv8_join_portion_kernel<UNIT, TILE>, dim3((unsigned)(p.slots * (UNIT / JOIN_ROWS)), (unsigned)p.nkv), dim3(256),
+                             0, stream, p);
 }
 
 #if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128

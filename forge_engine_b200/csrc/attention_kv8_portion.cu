@@ -672,7 +672,7 @@ int launch_portion(Kv8Attention p, cudaStream_t stream) {
   if (err != cudaSuccess) return (int)err;
   int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)p.slots, (unsigned)p.spans), dim3(THREADS), SMEM, stream, p);
   if (rc == 0 && p.spans > 1)
-    rc = launch_join<PORTION_UNIT, PORTION_TILE, true>(p, stream);
+    rc = launch_join_portion<PORTION_UNIT, PORTION_TILE>(p, stream);
   return rc;
 }
 

@@ -1913,7 +1913,7 @@ def kv8_lib(head_dim: int):
             raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
         p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
         fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
-        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, f, i, i, i, i, i, i, p, p, p]
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, i, i, p, p, p]
         fn.restype = c_int
         size.argtypes = [i, i, i, i, i, i]
         size.restype = ll
@@ -2068,15 +2068,17 @@ def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, 
 
 
 # What a block of the attention over an 8-bit cache costs on a B200, in microseconds, fitted to measured calls: (blocks the
-# GPU holds at once, a key tile of a block that has its SM to itself, the same where all SMs are full, a block beside its
-# tiles, joining the pieces of cut entries, of that each piece of the longest).  Single tokens: 8 requests of 2,048 keys
-# 17.7 us with 3 tiles a block (384 blocks), 21.4 with 2 (512: a second round), 26.2 with 8, 38 uncut; 48 requests in a
-# window of 4,096 94 uncut, 112 with 5.  Portions: 509 tokens behind 32,259 keys 426 us with 64 tiles a block (256 blocks),
-# 443 with 128 (128), 546 with 86 (192: the second round is half empty), 824 uncut.
-_KV8_SINGLE = (444, 1.75, 3.2, 2.2, 4.0, 0.05)
+# GPU holds at once, a key tile of a block where they share their SMs as cut entries do, the same where all SMs are full, a
+# block beside its tiles, joining the pieces of cut entries, of that each piece of the longest).  Up to 8 rows: 8 requests of
+# 2,048 keys 13.8 us with 4 tiles a block (320 blocks), 16.5 with 2 (576: a second round), 15.8 with 8, 23.5 uncut; 100,000
+# keys of one 45.6 with 24, 65.7 with 4.  9 to 16 rows: 48 requests in a window of 4,096 84 uncut, 116 with 4.  Portions:
+# 509 tokens behind 32,259 keys 421 us with 64 tiles a block (256 blocks), 433 with 128 (128), 538 with 86 (192: the second
+# round is half empty), 824 uncut.
+_KV8_FEW = (444, 1.3, 2.6, 3.3, 4.2, 0.04)
+_KV8_SINGLE = (444, 1.7, 2.4, 6.6, 6.8, 0.02)
 _KV8_PORTION = (148, 3.2, 3.2, 9.0, 8.0, 0.0)
 _KV8_PORTION_MMA = (296, 7.0, 9.0, 3.0, 6.0, 0.0)
-_KV8_SPANS = tuple(sorted({m << e for e in range(0, 22) for m in (2, 3)} | {1}))
+_KV8_SPANS = tuple(sorted({m << e for e in range(0, 24) for m in (2, 3)} | {1}))       # tiles of a block, and blocks of a unit
 
 
 @_functools.lru_cache(maxsize=4096)
@@ -2091,13 +2093,14 @@ def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int,
         elif rows:
             for row in range(0, rows, rows_of):
                 portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
-    return (*_kv8_cut(few, nkv, *_KV8_SINGLE), *_kv8_cut(single, nkv, *_KV8_SINGLE), *_kv8_cut(portion, nkv, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
+    return (*_kv8_cut(few, nkv, *_KV8_FEW), *_kv8_cut(single, nkv, *_KV8_SINGLE), *_kv8_cut(portion, nkv, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
 
 
 def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block: float, join: float, piece: float) -> tuple:
-    """(key tiles a block takes, blocks of the longest unit, rounded up to a power of two) for units of so many tiles per
-    kv head.  Lengths are rounded up to two and a half bits first and spans are powers of two or three times one, so that a
-    growing context changes the plan, and with it a captured step, seldom; the last block of a unit takes what is left."""
+    """(key tiles a block takes, blocks of the longest unit) for units of so many tiles per kv head.  Lengths are rounded up
+    to three bits first, and both numbers are powers of two or three times one, so that a growing context changes the plan,
+    and with it a captured step, seldom; the last block of a unit takes what is left.  (Rounding the blocks to powers of two
+    took 56.8 us instead of 45.6 for 100,000 keys: of 512 blocks 248 were empty, and the others lay unevenly.)"""
     if not tiles:
         return 1, 0
     counts: dict = {}
@@ -2120,7 +2123,7 @@ def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block
         if span == longest:
             break
     span = best[1]
-    return span, 1 << (-(-longest // span) - 1).bit_length()
+    return span, next(s for s in _KV8_SPANS if s >= -(-longest // span))
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -2160,5 +2163,5 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     _kv8_call(index, fn,
               (q.data_ptr(), q_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                block_table.data_ptr(), block_table.shape[1], page_size, num_pages, nkv, groups, cu_tokens.data_ptr(),
-               starts.data_ptr(), n_entries, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_span,
+               starts.data_ptr(), n_entries, max_new, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_span,
                portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")
