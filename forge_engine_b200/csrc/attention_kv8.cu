@@ -348,7 +348,9 @@ struct WarpRing {
 // bits down to 2^-11 of the row's largest element and what is smaller to within 2^-18 of it; the tensor core sums them
 // to within 6e-8 of the sum of magnitudes.  Values go in as half-precision numbers, 16 of their elements on the side of
 // 16, so an output comes out transposed too.  One sequence of 32768 keys, 32 heads on 8: 25.9 us, where 16 rows a
-// product took 28.1; eight of 2048: 16.0 and 17.8.
+// product took 28.1; eight of 2048: 16.0 and 17.8 (21.5 and 13.9 since the cuts and launches below).  32 sequences of
+// up to 8192 keys: 61 to 65 us, 0.70 of the copy peak; instructions issue in 47 % of the cycles, three warps a scheduler
+// (registers and rings allow 12 an SM) wait for one another's latencies, not for memory.
 struct RowQueries {
   unsigned b[2][D / 16];             // [part][four codes]
   float factor[2];                   // of rows 2t, 2t + 1: what a product is multiplied by to be a score in log2 units
@@ -558,8 +560,7 @@ __device__ __forceinline__ void finish_rows(const Kv8Attention& p, const Entry& 
 }
 
 // grid: (kv heads, entries, spans); a block takes `span` key tiles of an entry, warp w the keys 32 w .. 32 w + 31 of each.
-// Blocks past an entry's last piece come last: in between they left the SMs unevenly filled (32768 keys: 25.2 us with 40
-// spans of which 33 have keys).
+// Blocks past an entry's last piece come last.
 // Registers: for heads of up to 128, what three blocks an SM leave (their rings do not leave room for more).
 __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kernel(Kv8Attention p) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -754,7 +755,8 @@ int launch_blocks(Kernel kernel, const Kv8Attention& p, cudaStream_t stream) {
   if (p.spans == 1) return fe_launch_dependent(kernel, grid, dim3(THREADS), MMA_SMEM, stream, p);
   // Cut entries fill the SMs by count, so no block of theirs is to be placed while the kernel before still holds some of
   // them: as a dependent launch one token behind 32768 keys takes 21.3 to 25.2 us from one count of spans to the next,
-  // without 21.4 for all (48 uncut windows of 15 rows behind a cache write: 85.7 as a dependent launch, 87.3 without).
+  // without 21.4 for all, and a decode step of 16 requests of 4096 tokens through 8 layers 863 and 809.  (48 uncut windows of
+  // 15 rows behind a cache write: 85.7 as a dependent launch, 87.3 without.)
   kernel<<<grid, THREADS, MMA_SMEM, stream>>>(p);
   return (int)cudaGetLastError();
 }
@@ -805,14 +807,12 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
                                       int single_span, int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
                                       cudaStream_t stream) {
   if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
-  if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
+  if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || keep_first > 0x7fff0000 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
   if (few_spans < 0 || single_spans < 0 || portion_spans < 0 || few_span < 1 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
   if ((few_spans > 1 || single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
   if ((long long)num_pages * nkv > 0x7fffffffLL / page_size) return FE_ERR_TOO_LARGE;       // rows of a cache: 31 bits
   if (entries > 65535 || nkv > 65535 || (long long)total_tokens * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
-  if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) ||
-      q_stride % 4)
-    return FE_ERR_BAD_ALIGN;
+  if ((((uintptr_t)k | (uintptr_t)v) & 15) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) || q_stride % 4) return FE_ERR_BAD_ALIGN;
   Kv8Attention p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out;
   p.k = (const unsigned char*)k; p.v = (const unsigned char*)v; p.ks = (const unsigned char*)ks; p.vs = (const unsigned char*)vs;

@@ -2,23 +2,30 @@
 // 128 (-DFE_HEAD_DIM).  Formulas and layout: attention_kv8.cu, kv8.cuh.
 //
 //   block = two query tiles of 128 rows (row = token * G + head in group) of one (entry, kv head) and one piece of
-//           its keys, in tiles of 128 keys that both query tiles use
+//           its keys, in tiles of 128 keys that both query tiles use; one block an SM, 16 warps of 128 registers
 //   warps 0-3, 4-7   tile 0 and tile 1.  First its queries, as two e4m3 numbers each: a row times a power of two,
 //           rounded, and what the rounding left.  Together they hold bfloat16's 8 bits down to 2^-11 of the row's
 //           largest element, and what is smaller to within 2^-18 of it, so the scores are products of 8-bit numbers
-//           with the cached codes as they lie in their pages: keys are only copied.  Then softmax, a thread a row: scores from tensor memory times the keys' scales,
-//           mask, running maximum (moved only when it grows by more than 2^8), weights back over the scores as bfloat16.
-//           A tile is taken in halves of 64 keys: while a half is in the softmax the tensor core works on the other
-//   warps 8-15   copy the keys of a tile, and bring its values: 16-byte pieces of codes into registers a tile ahead,
+//           with the cached codes as they lie in their pages: keys are only copied.  Then softmax, a thread a row:
+//           scores from tensor memory times the keys' scales, mask, running maximum (moved only when it grows by more
+//           than 2^8), weights back over the scores as bfloat16.  A tile is taken in halves of 64 keys: while a half is
+//           in the softmax the tensor core works on the other
+//   warps 8-13   copy the keys of a tile, and bring its values: 16-byte pieces of codes into registers a tile ahead,
 //           code * 2^b as bfloat16 (exact) into the swizzled tile in shared memory
-//   warps 16, 17   issue the products of tile 0 and tile 1: O_x += P_x V with P from tensor memory, then in the weights'
+//   warps 14, 15   issue the products of tile 0 and tile 1: O_x += P_x V with P from tensor memory, then in the weights'
 //           place the scores S_x = Q_x K^T (both parts of the queries) of the next tile's half.  A thread that issues
 //           products waits for the tensor core most of the time: one for both tiles left the tensor core idle while it
 //           waited for weights (5,700 cycles a tile), and a softmax thread that did it held up its row's warp (10,000)
 //
 // Values are not left as 8-bit numbers, because then the weights would have to be: a weight as two e4m3 numbers costs
 // a softmax thread more than the 256 rows' share of converting a value.  Measured with keys converted like the
-// values: 7,700 cycles a tile, all of it the staging warps.
+// values: 7,700 cycles a tile, all of it the staging warps.  20 warps, of 96 and of 120 registers, were slower too.
+//
+// A tile takes 4,600 to 5,000 cycles (2.6 to 3.2 us), a block about 9 us beside its tiles (row tile, pages, first keys and
+// queries one after the other, the last products and stores): 2,048 tokens from the start 68 us, 509 behind 32,259
+// keys 435.  The tensor core works in 26 to 38 % of the cycles, the exponentials' unit in 27 to 39 %, instructions issue in
+// 49 to 55 %: what bounds a tile is the chain of a softmax warp's half (scores out, maximum, exponentials, weights
+// back), of which a scheduler holds two beside the staging warps; registers leave no room for a third.
 
 #include <cuda_fp16.h>
 

@@ -76,8 +76,9 @@ template <int E> __device__ __forceinline__ void store_some(bf16* dst, const flo
 // A group of LANES lanes (a power of two, at least D / 2E) takes a head's vector; a lane holds E pairs (a[i], b[i])
 // that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others pair up
 // (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 2E, so E pairs are two stretches of E elements.
-// E = 8 where rows and R allow 16-byte loads of bfloat16 (4,096 tokens of 32 + 16 heads of 128: 34.6 us with E = 4, whose
-// instructions were the limit), else 4.  Queries are not measured for a scale, values not normalised.
+// E = 8 where rows and R allow 16-byte loads of bfloat16, else 4.  Queries are not measured for a scale, values not
+// normalised.  4,096 tokens of 32 + 16 heads of 128: 24.2 us, 0.60 of the copy peak, instructions issued in 72 % of the
+// cycles (34.6 us with E = 4); 64 tokens in 32 bits 3.2, one 2.5, most of it the launch and the first loads.
 template <typename T, int LANES, int E>
 __global__ void __launch_bounds__(128, 8)
 kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__ q_out, int nq, const T* __restrict__ k,
@@ -215,8 +216,9 @@ __device__ __forceinline__ void kv8_put(float* dst, unsigned codes, float scale)
   *reinterpret_cast<float4*>(dst) = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
 }
 
-// A warp takes a token: neighbouring lanes write neighbouring 16 bytes of its rows (with 16 codes a thread, whose 64
-// bytes of output lay apart, 73,728 tokens of 4 heads of 64 in 32 bits took 25.6 us).
+// A warp takes a token: neighbouring lanes write neighbouring 16 bytes of its rows.  32-bit output of several contexts, 4
+// heads of 64, 95 MB in all: 21.7 us, 0.67 of the copy peak, warps waiting for their pages, scales and codes (with 16 codes
+// a thread, whose 64 bytes of output lay apart, 25.6 us).
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv8_read_kernel(Kv8Pages c, const int* __restrict__ positions, const int* __restrict__ token_entry, T* __restrict__ k_out,
@@ -268,13 +270,13 @@ int kv8_write_typed(const void* q, long long q_stride, bf16* q_out, int nq, cons
     return fe_launch_dependent(kernel, grid, dim3(128), 0, stream, (const T*)q, q_stride, q_out, nq, (const T*)k, k_stride,
                                (const T*)v, v_stride, q_weight, k_weight, eps, table, rot, positions, token_entry, c, status);
   };
-  switch (lanes) {
-    case 1: return launch(kv8_write_kernel<T, 1, E>);
-    case 2: return launch(kv8_write_kernel<T, 2, E>);
-    case 4: return launch(kv8_write_kernel<T, 4, E>);
-    case 8: return launch(kv8_write_kernel<T, 8, E>);
-    case 16: return launch(kv8_write_kernel<T, 16, E>);
-    default: return launch(kv8_write_kernel<T, 32, E>);
+  constexpr int LEAST = 8 / E;                  // of heads of 16; 256 take 16 times as many
+  switch (lanes / LEAST) {
+    case 1: return launch(kv8_write_kernel<T, LEAST, E>);
+    case 2: return launch(kv8_write_kernel<T, 2 * LEAST, E>);
+    case 4: return launch(kv8_write_kernel<T, 4 * LEAST, E>);
+    case 8: return launch(kv8_write_kernel<T, 8 * LEAST, E>);
+    default: return launch(kv8_write_kernel<T, 16 * LEAST, E>);
   }
 }
 

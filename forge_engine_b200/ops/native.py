@@ -7,8 +7,8 @@ a CUDA device or without the library these functions raise ``CUDAUnavailableErro
 
 from __future__ import annotations
 
+import bisect as _bisect
 import ctypes
-import functools as _functools
 import os as _os
 from ctypes import c_float, c_int, c_ulonglong, c_void_p
 
@@ -1892,6 +1892,7 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor, status: torch.Tensor, w
 KV8_CODES, KV8_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_FEW_ROWS, KV8_SINGLE_ROWS = 8, 16     # rows (new tokens x heads per kv head) of an entry that the kernels of single tokens take
 KV8_TILE = 128               # keys of a tile
+KV8_POSITIONS = 0x7fff0000   # a sequence's positions are below
 KV8_TC5_DIMS = (64, 128)     # head sizes whose portions the tcgen05 kernel takes
 
 _kv8_handles: dict = {}
@@ -2057,7 +2058,20 @@ def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window
     """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries (tuples): the key tiles a
     block takes of an entry and such blocks of the longest one, for entries with at most 8 rows (new tokens x heads per kv
     head), with 9 to 16, and the others; 0 blocks: there is no such entry.  Layers of one geometry share it."""
-    return _kv8_plan(tuple(entries), num_q_heads // num_kv_heads, num_kv_heads, head_dim, window or 0, keep_first or 0)
+    groups, window, keep_first = num_q_heads // num_kv_heads, window or 0, keep_first or 0
+    tc5 = head_dim in KV8_TC5_DIMS
+    rows_of = 256 if tc5 else 64
+    few, single, portion = [], [], []
+    for start, count in entries:
+        rows = count * groups
+        if 0 < rows <= KV8_SINGLE_ROWS:
+            tiles = _kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE) if window else -(-(start + count) // KV8_TILE)
+            (few if rows <= KV8_FEW_ROWS else single).append(tiles)
+        elif rows:
+            for row in range(0, rows, rows_of):
+                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
+    return (*_kv8_cut(few, num_kv_heads, *_KV8_FEW), *_kv8_cut(single, num_kv_heads, *_KV8_SINGLE),
+            *_kv8_cut(portion, num_kv_heads, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
 
 
 def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, tile: int) -> int:
@@ -2081,41 +2095,34 @@ _KV8_PORTION_MMA = (296, 7.0, 9.0, 3.0, 6.0, 0.0)
 _KV8_SPANS = tuple(sorted({m << e for e in range(0, 24) for m in (2, 3)} | {1}))       # tiles of a block, and blocks of a unit
 
 
-@_functools.lru_cache(maxsize=4096)
-def _kv8_plan(entries: tuple, groups: int, nkv: int, head_dim: int, window: int, keep_first: int) -> tuple:
-    tc5 = head_dim in KV8_TC5_DIMS
-    rows_of = 256 if tc5 else 64
-    few, single, portion = [], [], []
-    for start, count in entries:
-        rows = count * groups
-        if 0 < rows <= KV8_SINGLE_ROWS:
-            (few if rows <= KV8_FEW_ROWS else single).append(_kv8_tiles(start, 0, count - 1, window, keep_first, KV8_TILE))
-        elif rows:
-            for row in range(0, rows, rows_of):
-                portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
-    return (*_kv8_cut(few, nkv, *_KV8_FEW), *_kv8_cut(single, nkv, *_KV8_SINGLE), *_kv8_cut(portion, nkv, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
-
-
 def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block: float, join: float, piece: float) -> tuple:
     """(key tiles a block takes, blocks of the longest unit) for units of so many tiles per kv head.  Lengths are rounded up
     to three bits first, and both numbers are powers of two or three times one, so that a growing context changes the plan,
     and with it a captured step, seldom; the last block of a unit takes what is left.  (Rounding the blocks to powers of two
-    took 56.8 us instead of 45.6 for 100,000 keys: of 512 blocks 248 were empty, and the others lay unevenly.)"""
+    took 56.8 us instead of 45.6 for 100,000 keys, with 248 of 512 blocks empty.)"""
     if not tiles:
         return 1, 0
     counts: dict = {}
+    total = 0
     for t in tiles:
-        unit = 1 << max(0, t.bit_length() - 3)
-        t = -(-t // unit) * unit
+        shift = t.bit_length() - 3
+        if shift > 0:
+            t = -(-t >> shift) << shift
         counts[t] = counts.get(t, 0) + nkv
+        total += t * nkv
     longest = max(counts)
-    total = sum(t * n for t, n in counts.items())
     best = None
-    for span in _KV8_SPANS:
+    # more than sixteen rounds of blocks cost more than fewer
+    first = _bisect.bisect_left(_KV8_SPANS, min(longest, total / (16 * slots)))
+    for span in _KV8_SPANS[first:]:
         span = min(span, longest)
-        pieces = sum(n * -(-t // span) for t, n in counts.items())
-        rounds = -(-sum(n * (t // span + (1 if 2 * (t % span) >= span else 0)) for t, n in counts.items()) // slots)
-        cost = max(max(1, rounds) * (alone * span + block), (full * total + block * pieces) / slots)
+        pieces = whole = 0
+        for t, n in counts.items():
+            times, rest = divmod(t, span)
+            whole += n * (times + (2 * rest >= span))
+            pieces += n * (times + (rest > 0))
+        round_of = max(1, -(-whole // slots)) * (alone * span + block)
+        cost = max(round_of, (full * total + block * pieces) / slots)
         if span < longest:
             cost += join + piece * -(-longest // span)
         if best is None or cost < best[0]:
@@ -2123,7 +2130,8 @@ def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block
         if span == longest:
             break
     span = best[1]
-    return span, next(s for s in _KV8_SPANS if s >= -(-longest // span))
+    blocks = -(-longest // span)
+    return span, _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, blocks)]
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -2152,6 +2160,8 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out), (q,))
     few_span, few_spans, single_span, single_spans, portion_span, portion_spans = plan
     groups = num_q_heads // nkv
+    # what is past any position or token says no more than the last one, and goes into 32 bits
+    window, keep_first, max_new = min(window, KV8_POSITIONS), min(keep_first, KV8_POSITIONS), min(max_new, n)
     if max_new * groups <= KV8_SINGLE_ROWS:
         portion_spans = 0
     fn, size = kv8_lib(d)

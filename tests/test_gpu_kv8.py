@@ -357,6 +357,69 @@ def test_bad_token_counts_touch_nothing(native) -> None:
             assert int(status.item()) == 4 and bool((out == 7.0).all())
 
 
+@pytest.mark.parametrize("dim", [64, 32])
+@pytest.mark.parametrize("requests", [[(5, 1), (0, 1)], [(40, 30)]])
+def test_scales_lie_anywhere(native, dim, requests) -> None:
+    """Scales are bytes: pages of one token of one head, and views that begin at an odd address."""
+    heads, nkv, page = 2, 1, 1
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 2)
+    caches = list(to_device(cache))
+    for i in (2, 3):
+        room = torch.zeros(caches[i].numel() + 1, dtype=torch.uint8, device=DEV)
+        room[1:] = caches[i].view(torch.uint8).flatten()
+        caches[i] = room[1:].view(caches[i].shape).view(plain.SCALES)
+        assert caches[i].data_ptr() % 4 == 1
+    q = torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, caches=caches)
+    assert status == 0
+    check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
+    # written and read back there
+    kv = torch.randn((1, dim)).to(DEV)
+    word, at = status_word(), ints([3])
+    native.kv8_write(kv, kv, at, ints([0]), *caches, cache["table"].to(DEV), word)
+    outs = [torch.empty((1, nkv, dim), device=DEV) for _ in range(2)]
+    native.kv8_read(*caches, cache["table"].to(DEV), at, ints([0]), *outs, word)
+    codes, scales = plain.quantise(kv.cpu()[:, None])
+    assert int(word.item()) == 0
+    assert all(torch.equal(o.cpu().double(), codes * torch.exp2(scales.double() - 127)[..., None]) for o in outs)
+
+
+@pytest.mark.parametrize("requests", [[(200, 1)], [(200, 30)]])
+@pytest.mark.parametrize("window,keep", [(2 ** 40, 0), (2 ** 32 + 5, 3), (2 ** 31 - 1, 2 ** 31 - 1), (20, 2 ** 31 - 1), (20, 2 ** 32 + 1)])
+def test_windows_and_kept_tokens_past_every_position(native, requests, window, keep) -> None:
+    dim, heads, nkv, page = 64, 4, 2, 16
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 1)
+    q = torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    out, status = attend(native, cache, requests, q, window, keep, dim ** -0.5)
+    assert status == 0
+    check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 32])
+@pytest.mark.parametrize("entry,most", [(3, 1), (5, 3), (30, 20)])
+def test_an_entry_of_more_tokens_than_said_is_told(native, dim, entry, most) -> None:
+    """The call is sized by ``max_new``; an entry beyond it sets the status bit and nothing of it is written, cut or not."""
+    heads, nkv, page = 4, 2, 16
+    cache = plain.pool([300], nkv, dim, page, 1)
+    caches, table = to_device(cache), cache["table"].to(DEV)
+    q = torch.randn((entry + 8, heads * dim)).to(torch.bfloat16).to(DEV)
+    for plan in ((1, 3, 1, 3, 1, 3), (4, 1, 4, 1, 4, 1)):
+        out, status = torch.full_like(q, 7.0), status_word()
+        native.attention_kv8(q, *caches, table, ints([0, entry]), ints([300 - entry]), 1, most, heads, 0, 0, 1.0, out, status, plan)
+        assert int(status.item()) == 4 and bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("dim", [64, 32, 128])
+def test_three_hundred_heads_on_one(native, dim) -> None:
+    """One token's rows fill more than a row tile."""
+    requests, heads = [(40, 1), (130, 2), (0, 1)], 300
+    cache = plain.pool([s + n for s, n in requests], 1, dim, 16, 3)
+    q = torch.randn((6, heads * dim), generator=torch.Generator().manual_seed(8)).to(torch.bfloat16)
+    out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5)
+    assert status == 0
+    check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
+
+
 def test_written_read_and_attended_together(native) -> None:
     """A prompt in two portions, then single tokens, each written and attended, on a stream of its own; the cache read
     back is what the attention saw."""

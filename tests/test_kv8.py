@@ -124,3 +124,11 @@ def test_plans_cover_every_key(entries, window, keep) -> None:
             assert (spans > 0) == bool(mine) and span >= 1 and (not spans or spans // (spans & -spans) in (1, 3))
             if mine and not window:
                 assert span * spans * native.KV8_TILE >= max(mine)
+
+
+def test_plans_take_any_pairs_once() -> None:
+    want = native.kv8_plan([(700, 1), (3, 40)], 32, 8, 128)
+    assert native.kv8_plan(iter([[700, 1], [3, 40]]), 32, 8, 128) == want
+    assert native.kv8_plan(((700, 1), (3, 40)), 32, 8, 128, None, 0) == want
+    # a context that grows by a token at a time changes its plan at most four times while it doubles
+    assert len({native.kv8_plan([(n, 1)], 32, 8, 128) for n in range(4096, 8192)}) <= 5
