@@ -371,7 +371,7 @@ struct RowQueries {
     big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
     const bool finite = big < 0x7f800000u;
-    const int ex = finite ? kv8_exponent(big) : 0;
+    const int ex = finite ? kv8_row_exponent(big) : 0;
     const float down = __int_as_float((127 - ex) << 23);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
@@ -553,8 +553,8 @@ __device__ __forceinline__ void finish_rows(const Kv8Attention& p, const Entry& 
       const int token = r / p.groups, gq = r - token * p.groups;
       store4(p.out + ((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + gq) * D + d, out);
     } else {
-      *reinterpret_cast<float4*>(ws + piece_element<ROWS>(r, d)) = num;
-      if (d == 0) { ws[(size_t)ROWS * D + 2 * r] = big; ws[(size_t)ROWS * D + 2 * r + 1] = den; }
+      *reinterpret_cast<float4*>(ws + piece_element(p, r, d)) = num;
+      if (d == 0) { ws[(size_t)p.ws_rows * D + 2 * r] = big; ws[(size_t)p.ws_rows * D + 2 * r + 1] = den; }
     }
   }
 }
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kerne
     }
   }
   __syncthreads();
-  finish_rows(p, e, kvh, rows, pieces, acc, ml, p.ws + (((size_t)entry * p.nkv + kvh) * p.spans + piece) * ROWS * (D + 2));
+  finish_rows(p, e, kvh, rows, pieces, acc, ml, piece_sums(p, entry, kvh, piece));
 }
 
 // ---- 9 to 16 rows, any number of head sizes that are no whole 32s, portions of head sizes other than 64 and 128 ----
@@ -645,6 +645,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   int entry = slot, unit = 0;
   if constexpr (PORTION) {
     const Slot<UNIT> at(p, slot);
+    if (at.entry < 0) return;
     entry = at.entry;
     unit = at.unit;
   }
@@ -696,7 +697,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 2);
   }
-  float* ws = p.ws + (((size_t)slot * p.nkv + kvh) * p.spans + piece) * UNIT * (D + 2);
+  float* ws = piece_sums(p, slot, kvh, piece);
   if constexpr (PORTION) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -709,11 +710,11 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
         for (int c = 0; c < 2; ++c) {
           const int d = value_column(n, c, t);
           if (pieces == 1) store_row(p, e, kvh, row, d, s.o[n][2 * h + c] * inv);
-          else ws[piece_element<UNIT>(r, d)] = s.o[n][2 * h + c];
+          else ws[piece_element(p, r, d)] = s.o[n][2 * h + c];
         }
       if (pieces > 1 && t == 0) {
-        ws[(size_t)UNIT * D + 2 * r] = s.m[h];
-        ws[(size_t)UNIT * D + 2 * r + 1] = s.l[h];
+        ws[(size_t)p.ws_rows * D + 2 * r] = s.m[h];
+        ws[(size_t)p.ws_rows * D + 2 * r + 1] = s.l[h];
       }
     }
   } else {
@@ -764,21 +765,20 @@ int launch_blocks(Kernel kernel, const Kv8Attention& p, cudaStream_t stream) {
 // Entries with row_lo < rows <= row_hi, at most 16.
 int launch_single(Kv8Attention p, cudaStream_t stream) {
   p.slots = p.entries;
+  p.ws_rows = (single_rows(p.max_new, p.groups, p.row_hi) + 1) & ~1;
   int rc = 0;
 #if FE_HEAD_DIM % 32 == 0
   rc = p.row_hi <= 8 ? launch_blocks(attn_kv8_rows_kernel, p, stream) : launch_blocks(attn_kv8_mma_kernel<false>, p, stream);
 #else
   rc = launch_blocks(attn_kv8_mma_kernel<false>, p, stream);
 #endif
-  return rc || p.spans == 1 ? rc : launch_join<ROWS, KEYS>(p, stream);
+  return rc || p.spans == 1 ? rc : launch_join<KEYS>(p, stream);
 }
 
 #if FE_HEAD_DIM != 64 && FE_HEAD_DIM != 128
 int launch_portion(Kv8Attention p, cudaStream_t stream) {
   constexpr int UNIT = ROWS * WARPS;
-  const long long slots = portion_slots(p.entries, p.total_tokens, p.groups, UNIT);
-  if (slots > 65535) return FE_ERR_TOO_LARGE;
-  p.slots = (int)slots;
+  p.ws_rows = UNIT;
   const int rc = launch_blocks(attn_kv8_mma_kernel<true>, p, stream);
   return rc || p.spans == 1 ? rc : launch_join_portion<UNIT, KEYS>(p, stream);
 }
@@ -786,32 +786,40 @@ int launch_portion(Kv8Attention p, cudaStream_t stream) {
 
 }  // namespace
 
-// 32-bit numbers of workspace that `entries` of `total_tokens` tokens in all need, cut into `spans` pieces.
-FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int portion, int entries, int nkv, int groups, int total_tokens, int spans) {
-  if (spans <= 1) return 0;
+// 32-bit numbers of workspace that a call needs; the three kinds of entries use it one after the other.
+FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int entries, int max_new, int nkv, int groups, int few_spans, int single_spans,
+                                                      int portion_units, int portion_spans) {
 #if FE_HEAD_DIM == 64 || FE_HEAD_DIM == 128
-  const int unit = portion ? PORTION_UNIT : ROWS;
+  constexpr int UNIT = PORTION_UNIT;
 #else
-  const int unit = portion ? ROWS * WARPS : ROWS;
+  constexpr int UNIT = ROWS * WARPS;
 #endif
-  const long long slots = portion ? portion_slots(entries, total_tokens, groups, unit) : entries;
-  return slots * nkv * spans * unit * (D + 2);
+  auto single = [&](int spans, int row_hi) -> long long {
+    return spans > 1 ? (long long)entries * spans * ((single_rows(max_new, groups, row_hi) + 1) & ~1) : 0;
+  };
+  long long most = portion_spans > 1 ? (long long)portion_units * portion_spans * UNIT : 0;
+  if (single(few_spans, 8) > most) most = single(few_spans, 8);
+  if (single(single_spans, ROWS) > most) most = single(single_spans, ROWS);
+  return most * nkv * (D + 2);
 }
 
 // The entries of a step with at most 8 rows (new tokens x heads per kv head) if few_spans is above zero, those with 9 to 16
-// if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.
+// if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.  The portions' row tiles number at
+// most portion_units.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
                                       int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new, int total_tokens,
                                       int window, int keep_first, float scale, int few_span, int few_spans,
-                                      int single_span, int single_spans, int portion_span, int portion_spans, float* workspace, int* status,
+                                      int single_span, int single_spans, int portion_units, int portion_span, int portion_spans,
+                                      float* workspace, int* status,
                                       cudaStream_t stream) {
   if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || keep_first > 0x7fff0000 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
+  if (portion_spans > 0 && portion_units < 1) return FE_ERR_BAD_SHAPE;
   if (few_spans < 0 || single_spans < 0 || portion_spans < 0 || few_span < 1 || single_span < 1 || portion_span < 1) return FE_ERR_BAD_SHAPE;
   if ((few_spans > 1 || single_spans > 1 || portion_spans > 1) && workspace == nullptr) return FE_ERR_BAD_SHAPE;
   if ((long long)num_pages * nkv > 0x7fffffffLL / page_size) return FE_ERR_TOO_LARGE;       // rows of a cache: 31 bits
-  if (entries > 65535 || nkv > 65535 || (long long)total_tokens * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
+  if (entries > 65535 || portion_units > 65535 || nkv > 65535 || (long long)total_tokens * groups > 0x7fffffffLL) return FE_ERR_TOO_LARGE;
   if ((((uintptr_t)k | (uintptr_t)v) & 15) || ((uintptr_t)q & 7) || ((uintptr_t)out & 15) || q_stride % 4) return FE_ERR_BAD_ALIGN;
   Kv8Attention p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out;
@@ -821,7 +829,7 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   for (int s = 0; s < 31; ++s)
     if (page_size == 1 << s) p.page_shift = s;
   p.nkv = nkv; p.groups = groups; p.cu_tokens = cu_tokens; p.starts = starts; p.total_tokens = total_tokens;
-  p.entries = entries; p.max_new = max_new; p.slots = 0;
+  p.entries = entries; p.max_new = max_new; p.slots = 0; p.ws_rows = 0;
   p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.ws = workspace;
   if (few_spans > 0) {
@@ -835,7 +843,7 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
     if (rc) return rc;
   }
   if (portion_spans > 0) {
-    p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans;
+    p.row_lo = ROWS; p.row_hi = 0x7fffffff; p.span = portion_span; p.spans = portion_spans; p.slots = portion_units;
     const int rc = launch_portion(p, stream);
     if (rc) return rc;
   }

@@ -28,8 +28,9 @@ struct Kv8Attention {
   int row_lo, row_hi;      // entries with row_lo < rows <= row_hi
   int span, spans;         // a block takes `span` key tiles of a unit; the grid holds `spans` of them
   int entries, max_new;    // max_new: the most tokens an entry has
-  int slots;               // row tiles of all entries, at most: see Slot
-  float* ws;               // [slots, nkv, spans][rows of a unit x (D + 2)]: see piece_element
+  int slots;               // single tokens: entries; portions: row tiles of all of them (see Slot)
+  int ws_rows;             // rows of a unit, at most; even
+  float* ws;               // [slots, nkv, spans][ws_rows x (D + 2)]: see piece_element
 };
 
 // The key tiles (of TILE keys) that the rows [row0, row0 + n) of an entry see: first the tiles that hold kept
@@ -72,23 +73,37 @@ __device__ __forceinline__ int key_page(const Kv8Attention& p, const int* table,
   return key < key_end && logical < p.max_pages ? __ldg(table + logical) : -1;
 }
 
-// Which row tile of which entry a block takes.  Entry e's tiles of UNIT rows are slots floor(cu[e] G / UNIT) + e on: they
-// never meet the next entry's, and there are no more slots than total tokens * G / UNIT + entries.  A warp finds the
-// entry, 32 of them at a time.
+// Which row tile of which entry a block takes: the tiles of UNIT rows of the entries with more than row_lo rows, one entry
+// after another; entry -1 past the last one.  A warp finds it, 32 entries at a time.  Entries that cannot be have one
+// tile, whose block says so.
 template <int UNIT> struct Slot {
   int entry, unit;
-  __device__ __forceinline__ Slot(const Kv8Attention& p, int slot) {
+  __device__ __forceinline__ Slot(const Kv8Attention& p, int slot) : entry(-1), unit(0) {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int e0 = 0; e0 < p.entries; e0 += 32) {
       const int e = e0 + lane;
-      const bool is = e < p.entries && (int)((long long)p.cu_tokens[e] * p.groups / UNIT) + e <= slot;
-      const unsigned votes = __ballot_sync(0xffffffffu, is);
-      before += __popc(votes);
-      if (votes != 0xffffffffu) break;
+      int mine = 0;
+      if (e < p.entries) {
+        const long long rows = ((long long)p.cu_tokens[e + 1] - p.cu_tokens[e]) * p.groups;
+        const bool can_be = rows >= 0 && rows <= (long long)p.total_tokens * p.groups;
+        mine = !can_be ? 1 : rows > p.row_lo ? (int)((rows + UNIT - 1) / UNIT) : 0;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int left = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += left;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + upto > slot);
+      if (past != 0u) {
+        const int at = __ffs(past) - 1;
+        entry = e0 + at;
+        unit = slot - before - __shfl_sync(0xffffffffu, upto - mine, at);
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    entry = max(before - 1, 0);
-    unit = slot - ((int)((long long)p.cu_tokens[entry] * p.groups / UNIT) + entry);
   }
 };
 
@@ -118,13 +133,12 @@ __device__ __forceinline__ float piece_share(float m, float l, float big) {
 
 // Element (row r of the unit, column d) of a piece's sums: stretches of eight columns, the rows' stretches side by
 // side, so that a thread that owns a row stores 32 bytes and its warp 1 KB in a line.  M and l follow the sums.
-template <int UNIT> __device__ __forceinline__ size_t piece_element(int r, int d) {
-  return ((size_t)(d >> 3) * UNIT + r) * 8 + (d & 7);
+__device__ __forceinline__ size_t piece_element(const Kv8Attention& p, int r, int d) {
+  return ((size_t)(d >> 3) * p.ws_rows + r) * 8 + (d & 7);
 }
-
-// Row tiles of UNIT rows of a call's portions, at most.
-inline long long portion_slots(int entries, int total_tokens, int groups, int unit) {
-  return (long long)total_tokens * groups / unit + entries;
+__device__ __forceinline__ size_t piece_size(const Kv8Attention& p) { return (size_t)p.ws_rows * (D + 2); }
+__device__ __forceinline__ float* piece_sums(const Kv8Attention& p, int slot, int kvh, int piece) {
+  return p.ws + (((size_t)slot * p.nkv + kvh) * p.spans + piece) * piece_size(p);
 }
 
 // Joins the pieces of a single token's rows.  A row may have a hundred of them: a block a row, its eight warps every
@@ -133,7 +147,7 @@ inline long long portion_slots(int entries, int total_tokens, int groups, int un
 // grid: (entries * rows of an entry, kv heads)
 constexpr int JOIN_WARPS = 8;
 
-template <int UNIT, int TILE>
+template <int TILE>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Attention p, int rows_most) {
   constexpr int COLUMNS = D >= 128 ? 4 : 2, LANES_D = 32 * COLUMNS;
   constexpr int PASSES = (D + LANES_D - 1) / LANES_D;
@@ -147,9 +161,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
   const Walk<TILE> walk(p, e.start, 0, rows);
   const int pieces = pieces_of(p, walk.count);
   if (pieces == 1) return;
-  const size_t step = (size_t)UNIT * (D + 2);
-  const float* ws = p.ws + ((size_t)entry * p.nkv + kvh) * p.spans * step;
-  const float* ml = ws + (size_t)UNIT * D + 2 * r;
+  const size_t step = piece_size(p);
+  const float* ws = piece_sums(p, entry, kvh, 0);
+  const float* ml = ws + (size_t)p.ws_rows * D + 2 * r;
   float big = -INFINITY;
   for (int s = lane; s < pieces; s += 32) big = fmaxf(big, ml[s * step]);
   big = warp_max(big);
@@ -177,7 +191,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
         if (D % LANES_D == 0 || d < D) {
 #pragma unroll
           for (int c = 0; c < COLUMNS; c += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(src + piece_element<UNIT>(r, d + c));
+            const float2 x = *reinterpret_cast<const float2*>(src + piece_element(p, r, d + c));
             num[i][c] += x.x * f;
             num[i][c + 1] += x.y * f;
           }
@@ -214,6 +228,7 @@ __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention
   pdl_wait();
   const int slot = blockIdx.x / BLOCKS, kvh = blockIdx.y;
   const Slot<UNIT> at(p, slot);
+  if (at.entry < 0) return;
   const Entry e(p, at.entry);
   const int rows = e.n_new * p.groups, row0 = at.unit * UNIT, r0 = (blockIdx.x - slot * BLOCKS) * JOIN_ROWS;
   if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 + r0 >= rows) return;
@@ -221,11 +236,11 @@ __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention
   const Walk<TILE> walk(p, e.start, row0, rows_end);
   const int pieces = pieces_of(p, walk.count);
   if (pieces == 1) return;
-  const size_t step = (size_t)UNIT * (D + 2);
-  const float* ws = p.ws + ((size_t)slot * p.nkv + kvh) * p.spans * step;
+  const size_t step = piece_size(p);
+  const float* ws = piece_sums(p, slot, kvh, 0);
   const int i = threadIdx.x, r = r0 + (i & 7) + 8 * (i / (8 * STRETCHES)), d = 8 * ((i >> 3) % STRETCHES);
   if (i >= JOIN_ROWS * STRETCHES || row0 + r >= rows_end) return;
-  const float* ml = ws + (size_t)UNIT * D + 2 * r;
+  const float* ml = ws + (size_t)p.ws_rows * D + 2 * r;
   float big = -INFINITY, den = 0.f, num[8];
 #pragma unroll
   for (int c = 0; c < 8; ++c) num[c] = 0.f;
@@ -239,7 +254,7 @@ __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention
       a[s] = b[s] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (s0 + s < pieces) {
         of[s] = *reinterpret_cast<const float2*>(ml + (s0 + s) * step);
-        const float4* src = reinterpret_cast<const float4*>(ws + (s0 + s) * step + piece_element<UNIT>(r, d));
+        const float4* src = reinterpret_cast<const float4*>(ws + (s0 + s) * step + piece_element(p, r, d));
         a[s] = src[0];
         b[s] = src[1];
       }
@@ -267,12 +282,14 @@ __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention
   store4(to + 4, num + 4);
 }
 
-template <int UNIT, int TILE>
+// Rows that an entry of a call of single tokens has at most.
+inline int single_rows(long long max_new, int groups, int row_hi) { return max_new * groups < row_hi ? (int)(max_new * groups) : row_hi; }
+
+template <int TILE>
 inline int launch_join(const Kv8Attention& p, cudaStream_t stream) {
-  const long long most = (long long)p.max_new * p.groups;
-  const int rows = most < p.row_hi ? (int)most : p.row_hi;
-  return fe_launch_dependent(attn_kv8_join_kernel<UNIT, TILE>, dim3((unsigned)(p.slots * rows), (unsigned)p.nkv), dim3(32 * JOIN_WARPS), 0,
-                             stream, p, rows);
+  const int rows = single_rows(p.max_new, p.groups, p.row_hi);
+  return fe_launch_dependent(attn_kv8_join_kernel<TILE>, dim3((unsigned)(p.slots * rows), (unsigned)p.nkv), dim3(32 * JOIN_WARPS), 0, stream, p,
+                             rows);
 }
 
 template <int UNIT, int TILE>

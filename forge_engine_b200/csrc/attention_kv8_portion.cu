@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   // blocks start in the order of x, y, z: the row tiles that see most keys first
   const int kvh = blockIdx.x, slot = gridDim.y - 1 - blockIdx.y, piece = blockIdx.z;
   const Slot<PORTION_UNIT> at(p, slot);
+  if (at.entry < 0) return;
   const Entry e(p, at.entry);
   const int rows = e.n_new * p.groups, row0 = at.unit * PORTION_UNIT;
   if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
 #pragma unroll
           for (int o = Q_LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
           const bool finite = big < 0x7f800000u;
-          const int ex = finite ? kv8_exponent(big) : 0;
+          const int ex = finite ? kv8_row_exponent(big) : 0;
           const float down = __int_as_float((127 - ex) << 23);
           unsigned hi[4], lo[4];
 #pragma unroll
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
     if (ok) {
       const int ur = x * TILE_ROWS + r;
       const float by = pieces > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* ws = p.ws + (((size_t)slot * p.nkv + kvh) * p.spans + piece) * (size_t)PORTION_UNIT * (D + 2);
+      float* ws = piece_sums(p, slot, kvh, piece);
       // a finished warp's 32 rows pass through its queries' place, so that whole rows go out
       unsigned char* rows_here = q_tiles + x * 2 * CODE_TILE + quarter * 32 * D * 2;
 #pragma unroll 1
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
             const int chunk = (c + j) >> 3;
             store8(reinterpret_cast<bf16*>(rows_here + lane * D * 2 + ((chunk ^ (lane & 7)) << 4)), o);
           } else if (row_valid) {
-            store8(ws + piece_element<PORTION_UNIT>(ur, c + j), o);
+            store8(ws + piece_element(p, ur, c + j), o);
           }
         }
       }
@@ -652,8 +653,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
               *reinterpret_cast<const uint4*>(rows_here + n * D * 2 + ((chunk ^ (n & 7)) << 4));
         }
       } else if (row_valid) {
-        ws[(size_t)PORTION_UNIT * D + 2 * ur] = m;
-        ws[(size_t)PORTION_UNIT * D + 2 * ur + 1] = l;
+        ws[(size_t)p.ws_rows * D + 2 * ur] = m;
+        ws[(size_t)p.ws_rows * D + 2 * ur + 1] = l;
       }
     }
   }
@@ -672,9 +673,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
 namespace kv8 {
 
 int launch_portion(Kv8Attention p, cudaStream_t stream) {
-  const long long slots = portion_slots(p.entries, p.total_tokens, p.groups, PORTION_UNIT);
-  if (slots > 65535 || p.spans > 65535) return FE_ERR_TOO_LARGE;
-  p.slots = (int)slots;
+  if (p.spans > 65535) return FE_ERR_TOO_LARGE;
+  p.ws_rows = PORTION_UNIT;
   const cudaError_t err = cudaFuncSetAttribute(attn_kv8_portion_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
   if (err != cudaSuccess) return (int)err;
   int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)p.slots, (unsigned)p.spans), dim3(THREADS), SMEM, stream, p);

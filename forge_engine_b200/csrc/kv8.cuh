@@ -32,6 +32,11 @@ __device__ __forceinline__ int kv8_exponent(unsigned bits) {
   const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, KV8_LEAST), KV8_MOST);
 }
+// The same for a row that is not stored: every size a 32-bit number has, as far as 2^e and 2^-e are ones (rows below
+// 448 * 2^-120 lose bits).
+__device__ __forceinline__ int kv8_row_exponent(unsigned bits) {
+  return max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -120);
+}
 
 // two codes of two 32-bit numbers, rounded to nearest even, `lo` in the low byte
 __device__ __forceinline__ unsigned short kv8_codes(float lo, float hi) {

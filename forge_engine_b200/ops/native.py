@@ -1914,9 +1914,9 @@ def kv8_lib(head_dim: int):
             raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
         p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
         fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
-        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, i, i, p, p, p]
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, i, i, i, p, p, p]
         fn.restype = c_int
-        size.argtypes = [i, i, i, i, i, i]
+        size.argtypes = [i, i, i, i, i, i, i, i]
         size.restype = ll
         got = _kv8_handles[head_dim] = (fn, size)
     return got
@@ -2057,7 +2057,8 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
 def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window: int | None = None, keep_first: int = 0) -> tuple:
     """The host's decision for ``attention_kv8``, from the (cached, new) token counts of a step's entries (tuples): the key tiles a
     block takes of an entry and such blocks of the longest one, for entries with at most 8 rows (new tokens x heads per kv
-    head), with 9 to 16, and the others; 0 blocks: there is no such entry.  Layers of one geometry share it."""
+    head), with 9 to 16, and the others; 0 blocks: there is no such entry; then the others' row tiles, at most.  Layers of one
+    geometry share it."""
     groups, window, keep_first = num_q_heads // num_kv_heads, window or 0, keep_first or 0
     tc5 = head_dim in KV8_TC5_DIMS
     rows_of = 256 if tc5 else 64
@@ -2070,8 +2071,12 @@ def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window
         elif rows:
             for row in range(0, rows, rows_of):
                 portion.append(_kv8_tiles(start, row // groups, (min(rows, row + rows_of) - 1) // groups, window, keep_first, KV8_TILE))
-    return (*_kv8_cut(few, num_kv_heads, *_KV8_FEW), *_kv8_cut(single, num_kv_heads, *_KV8_SINGLE),
-            *_kv8_cut(portion, num_kv_heads, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA)))
+    few_cut = _kv8_cut(few, num_kv_heads, *_KV8_FEW) if few else (1, 0)
+    single_cut = _kv8_cut(single, num_kv_heads, *_KV8_SINGLE) if single else (1, 0)
+    if not portion:
+        return (*few_cut, *single_cut, 1, 0, 0)
+    cut = _kv8_cut(portion, num_kv_heads, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA))
+    return (*few_cut, *single_cut, *cut, _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, len(portion))])
 
 
 def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, tile: int) -> int:
@@ -2100,8 +2105,6 @@ def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block
     to three bits first, and both numbers are powers of two or three times one, so that a growing context changes the plan,
     and with it a captured step, seldom; the last block of a unit takes what is left.  (Rounding the blocks to powers of two
     took 56.8 us instead of 45.6 for 100,000 keys, with 248 of 512 blocks empty.)"""
-    if not tiles:
-        return 1, 0
     counts: dict = {}
     total = 0
     for t in tiles:
@@ -2111,27 +2114,37 @@ def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block
         counts[t] = counts.get(t, 0) + nkv
         total += t * nkv
     longest = max(counts)
-    best = None
-    # more than sixteen rounds of blocks cost more than fewer
-    first = _bisect.bisect_left(_KV8_SPANS, min(longest, total / (16 * slots)))
-    for span in _KV8_SPANS[first:]:
-        span = min(span, longest)
-        pieces = whole = 0
-        for t, n in counts.items():
-            times, rest = divmod(t, span)
-            whole += n * (times + (2 * rest >= span))
-            pieces += n * (times + (rest > 0))
-        round_of = max(1, -(-whole // slots)) * (alone * span + block)
-        cost = max(round_of, (full * total + block * pieces) / slots)
-        if span < longest:
-            cost += join + piece * -(-longest // span)
-        if best is None or cost < best[0]:
-            best = (cost, span)
-        if span == longest:
+    units = tuple(counts.items())
+    least = full * total / slots
+    best, span = None, 0
+    for s in _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, total // (8 * slots)):]:      # more than eight rounds cost more than fewer
+        if s >= longest:
             break
-    span = best[1]
-    blocks = -(-longest // span)
-    return span, _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, blocks)]
+        pieces = whole = halves = 0
+        for t, n in units:
+            times, rest = divmod(t, s)
+            whole += n * times
+            if rest:
+                pieces += n
+                if rest + rest >= s:
+                    halves += n
+        pieces += whole
+        whole += halves
+        rounds = -(-whole // slots) or 1
+        cost, spread = rounds * (alone * s + block), least + block * pieces / slots
+        done = rounds == 1 and cost >= spread          # longer ones only leave SMs empty
+        if spread > cost:
+            cost = spread
+        cost += join + piece * -(-longest // s)
+        if best is None or cost < best:
+            best, span = cost, s
+        if done:
+            break
+    whole = sum(n for t, n in units if 2 * t >= longest)
+    uncut = max(-(-whole // slots) * (alone * longest + block), least + block * len(tiles) * nkv / slots)
+    if best is None or uncut < best:
+        return longest, 1
+    return span, _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, -(-longest // span))]
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -2158,7 +2171,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             or block_table.shape[0] < n_entries):
         raise UnsupportedShapeError("cu_tokens holds entries + 1 int32 numbers, starts one an entry, block_table a row")
     index = _kv8_device((k_cache, v_cache, k_scale, v_scale, block_table, status, cu_tokens, starts, out), (q,))
-    few_span, few_spans, single_span, single_spans, portion_span, portion_spans = plan
+    few_span, few_spans, single_span, single_spans, portion_span, portion_spans, portion_units = plan
     groups = num_q_heads // nkv
     # what is past any position or token says no more than the last one, and goes into 32 bits
     window, keep_first, max_new = min(window, KV8_POSITIONS), min(keep_first, KV8_POSITIONS), min(max_new, n)
@@ -2168,10 +2181,10 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     workspace = None
     if few_spans > 1 or single_spans > 1 or portion_spans > 1:
         # the pieces of a cut entry meet in a buffer of the call's own: calls on other streams, and captured ones, have theirs
-        numbers = max(size(0, n_entries, nkv, groups, n, max(few_spans, single_spans)), size(1, n_entries, nkv, groups, n, portion_spans))
+        numbers = size(n_entries, max_new, nkv, groups, few_spans, single_spans, portion_units, portion_spans)
         workspace = torch.empty(numbers, dtype=torch.float32, device=q.device)
     _kv8_call(index, fn,
               (q.data_ptr(), q_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                block_table.data_ptr(), block_table.shape[1], page_size, num_pages, nkv, groups, cu_tokens.data_ptr(),
-               starts.data_ptr(), n_entries, max_new, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_span,
-               portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")
+               starts.data_ptr(), n_entries, max_new, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_units,
+               portion_span, portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")

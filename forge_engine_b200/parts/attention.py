@@ -369,13 +369,14 @@ class GQAttention(Mixer):
 
     def _attend_eight_bit(self, x, batch, cache: CacheView):
         """The plain layer over an 8-bit cache: one kernel norms and rotates q and k and quantises k and v into their
-        pages, and the attention reads the codes.  Up to 64 tokens the projection leaves 32-bit sums."""
+        pages, and the attention reads the codes.  Up to 64 tokens the projection leaves 32-bit sums (a position encoding that
+        rewrites q and k itself gets the engine's type, as everywhere)."""
         caches = (*cache.kv, *cache.scales)
         table = batch.group_tables[cache.group]
         q_end, k_end = self.nq * self.d, (self.nq + self.nkv) * self.d
         with self.ctx.section("mixer.qkv_rope_cache"):
-            qkv = self.qkv_proj(x, out_dtype=torch.float32 if self.qkv_proj._tc5_ok(x) else None)
             rotary, angles = self.position.rotary(), None
+            qkv = self.qkv_proj(x, out_dtype=torch.float32 if rotary is not None and self.qkv_proj._tc5_ok(x) else None)
             if rotary is None:
                 self.position.apply(qkv, self.nq, self.nkv, self.d, batch)
             elif rotary[1]:

@@ -268,7 +268,7 @@ def test_attention_cut_into_pieces(native, dim, requests) -> None:
     cache = plain.pool([s + n for s, n in requests], nkv, dim, page, dim)
     g = torch.Generator().manual_seed(4)
     q = (torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=g) * 2).to(torch.bfloat16)
-    for spans in ((1, 16, 1, 16, 1, 16), (2, 8, 2, 8, 3, 8), (3, 4, 3, 4, 2, 2), (1, 2, 1, 2, 1, 2), (100, 1, 100, 1, 100, 1)):
+    for spans in ((1, 16, 1, 16, 1, 16, 8), (2, 8, 2, 8, 3, 8, 12), (3, 4, 3, 4, 2, 2, 8), (1, 2, 1, 2, 1, 2, 8), (100, 1, 100, 1, 100, 1, 8)):
         for window, keep in ((0, 0), (200, 20)):
             out, status = attend(native, cache, requests, q, window, keep, dim ** -0.5, plan=spans)
             assert status == 0
@@ -297,6 +297,21 @@ def test_attention_with_scales_of_every_size(native, dim) -> None:
         out, status = attend(native, cache, requests, scaled, 0, 0, dim ** -0.5)
         assert status == 0
         check_attention(cache, requests, scaled, out, 0, 0, dim ** -0.5, large_scores=factor > 1)
+
+
+@pytest.mark.parametrize("dim", [128, 64, 96])
+@pytest.mark.parametrize("up,down", [(75, -72), (-71, 71), (100, -73), (-90, 71)])
+def test_queries_far_from_one(native, dim, up, down) -> None:
+    """Queries beyond the scales a cached vector can have, against keys at the other end."""
+    heads, nkv, page, requests = 8, 2, 16, [(100, 1), (70, 4), (60, 50)]
+    g = torch.Generator().manual_seed(dim)
+    values = [tuple(torch.randn((s + n, nkv, dim), generator=g, dtype=torch.float64) * f for f in (2.0 ** down, 1.0)) for s, n in requests]
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5, values=values)
+    q = (torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=g, dtype=torch.float64) * 2.0 ** up).to(torch.bfloat16)
+    scale = dim ** -0.5 * 2.0 ** -(up + down)
+    out, status = attend(native, cache, requests, q, 0, 0, scale)
+    assert status == 0
+    check_attention(cache, requests, q, out, 0, 0, scale)
 
 
 @pytest.mark.parametrize("dim,requests", [(128, [(90, 1), (100, 4), (0, 1)]), (128, [(20, 100), (0, 70)]), (64, [(20, 150)]), (32, [(20, 40)])])
@@ -351,7 +366,7 @@ def test_bad_token_counts_touch_nothing(native) -> None:
     caches = to_device(cache)
     q = torch.randn((4, heads * dim)).to(torch.bfloat16).to(DEV)
     for ends, starts in (([0, 5, 6], [0, 0]), ([-1, 2, 3], [0, 0]), ([3, 1, 1], [0, 0]), ([0, 1, 2], [-5, -1])):
-        for plan in ((1, 2, 1, 2, 1, 2), (4, 1, 4, 1, 4, 1)):
+        for plan in ((1, 2, 1, 2, 1, 2, 2), (4, 1, 4, 1, 4, 1, 2)):
             out, status = torch.full_like(q, 7.0), status_word()
             native.attention_kv8(q, *caches, cache["table"].to(DEV), ints(ends), ints(starts), 1, 5, heads, 0, 0, 1.0, out, status, plan)
             assert int(status.item()) == 4 and bool((out == 7.0).all())
@@ -403,10 +418,26 @@ def test_an_entry_of_more_tokens_than_said_is_told(native, dim, entry, most) -> 
     cache = plain.pool([300], nkv, dim, page, 1)
     caches, table = to_device(cache), cache["table"].to(DEV)
     q = torch.randn((entry + 8, heads * dim)).to(torch.bfloat16).to(DEV)
-    for plan in ((1, 3, 1, 3, 1, 3), (4, 1, 4, 1, 4, 1)):
+    for plan in ((1, 3, 1, 3, 1, 3, 2), (4, 1, 4, 1, 4, 1, 2)):
         out, status = torch.full_like(q, 7.0), status_word()
         native.attention_kv8(q, *caches, table, ints([0, entry]), ints([300 - entry]), 1, most, heads, 0, 0, 1.0, out, status, plan)
         assert int(status.item()) == 4 and bool((out == 7.0).all())
+
+
+def test_a_portion_behind_a_long_context_among_many_single_tokens(native) -> None:
+    """Row tiles are counted over the portions alone: more entries than a warp looks at in a step, portions in front, in the
+    middle and last, empty entries between; the pieces' buffer grows with the portions, not with the entries."""
+    dim, heads, nkv, page = 128, 8, 2, 16
+    requests = [(7, 9)] + [(30 + i, 1) for i in range(40)] + [(1500, 150), (0, 0), (3, 3)] + [(60, 1)] * 30 + [(700, 70)]
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5)
+    q = (torch.randn((sum(n for _, n in requests) + 2, heads * dim), generator=torch.Generator().manual_seed(2)) * 2).to(torch.bfloat16)
+    made = native.kv8_plan(requests, heads, nkv, dim, 0, 0)
+    assert made[6] == 6                          # 1 + 3 + 2
+    for cut in (made, (1, 4, 1, 4, 2, 8, 6)):
+        out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, plan=cut)
+        assert status == 0
+        check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
+    assert native.kv8_lib(dim)[1](len(requests), 150, nkv, 4, 4, 4, 6, 8) == 6 * nkv * 8 * 256 * (dim + 2)
 
 
 @pytest.mark.parametrize("dim", [64, 32, 128])
@@ -473,7 +504,7 @@ def test_two_captured_graphs_and_eager_calls_between(native) -> None:
         args = (q.to(DEV), *to_device(cache), cache["table"].to(DEV), ints(ends), ints(s for s, _ in requests), len(requests),
                 max(n for _, n in requests), heads, 0, 0, dim ** -0.5)
         cases.append((cache, requests, q, args, torch.zeros(q.shape, dtype=torch.bfloat16, device=DEV), status_word()))
-    plan = (2, 8, 2, 8, 2, 8)
+    plan = (2, 8, 2, 8, 2, 8, 4)
     graphs, streams = [], []
     for cache, requests, q, args, out, status in cases:
         native.attention_kv8(*args, out, status, plan)

@@ -35,7 +35,7 @@ def attention_args(**other):
     args = {**caches(), "q": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "block_table": torch.zeros((2, 3), dtype=torch.int32),
             "cu_tokens": torch.tensor([0, 1, 6], dtype=torch.int32), "starts": torch.zeros(2, dtype=torch.int32), "n_entries": 2,
             "max_new": 5, "num_q_heads": HEADS, "window": None, "keep_first": 0, "scale": 1.0,
-            "out": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "status": torch.zeros(1, dtype=torch.int32), "plan": (1, 1, 1, 1, 1, 1)}
+            "out": torch.zeros((N, HEADS * DIM), dtype=torch.bfloat16), "status": torch.zeros(1, dtype=torch.int32), "plan": (1, 1, 1, 1, 1, 1, 1)}
     return {**args, **other}
 
 
@@ -118,12 +118,14 @@ def test_plans_cover_every_key(entries, window, keep) -> None:
     for heads, nkv, dim in ((32, 8, 128), (4, 4, 64), (16, 1, 96)):
         plan = native.kv8_plan(entries, heads, nkv, dim, window, keep)
         groups = heads // nkv
-        kinds = [(lambda r: 0 < r <= 8, plan[:2]), (lambda r: 8 < r <= 16, plan[2:4]), (lambda r: r > 16, plan[4:])]
+        kinds = [(lambda r: 0 < r <= 8, plan[:2]), (lambda r: 8 < r <= 16, plan[2:4]), (lambda r: r > 16, plan[4:6])]
         for is_kind, (span, spans) in kinds:
             mine = [start + n for start, n in entries if is_kind(n * groups)]
             assert (spans > 0) == bool(mine) and span >= 1 and (not spans or spans // (spans & -spans) in (1, 3))
             if mine and not window:
                 assert span * spans * native.KV8_TILE >= max(mine)
+        rows_of = 256 if dim in (64, 128) else 64
+        assert plan[6] >= sum(-(-n * groups // rows_of) for _, n in entries if n * groups > 16)
 
 
 def test_plans_take_any_pairs_once() -> None:
