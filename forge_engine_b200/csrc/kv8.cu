@@ -73,14 +73,88 @@ template <int E> __device__ __forceinline__ void store_some(bf16* dst, const flo
   if constexpr (E == 8) store8(dst, v); else store4(dst, v);
 }
 
+// Keys that were normalised or rotated are rounded to four bits behind a 32-bit computation, so an element whose 32-bit
+// error spans the middle between two codes could take the wrong one (4,096 tokens of 8 heads: about 5 of 4.2 million).
+// The writer converts the two ends of that span, and where they differ anywhere in a head (about one in thirty) the
+// head's lanes take it again in 64 bits, from the row as it lies in memory: codes and scale are those of exact arithmetic.
+struct Kv8Exact {
+  unsigned codes[4];               // of the lane's E elements from ia on, then from ib on
+  int e8;
+};
+// a 64-bit number as a 32-bit one whose last bit says that something is missing: rounding it to fewer bits rounds once
+__device__ __forceinline__ float kv8_odd(double x) {
+  const float y = __double2float_rz(x);
+  return (double)y == x ? y : __int_as_float(__float_as_int(y) | 1);
+}
+template <typename T, int LANES, int E>
+__device__ __forceinline__ Kv8Exact kv8_exact(const T* x, const float* w, const float2* turn, int ia, int ib, bool mine, float eps, int D,
+                                           unsigned group) {
+  float a[E], b[E];
+  Held<E, T> held;
+#pragma unroll
+  for (int e = 0; e < E; ++e) a[e] = b[e] = 0.f;
+  if (mine) {
+    held.load(x + ia);
+    held.numbers(a);
+    held.load(x + ib);
+    held.numbers(b);
+  }
+  double inv = 1.0;
+  if (w != nullptr) {
+    double ss = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss = fma((double)a[e], (double)a[e], fma((double)b[e], (double)b[e], ss));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+    inv = rsqrt(ss / D + (double)eps);
+  }
+  double p[E], r[E];
+  unsigned big = 0u;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    p[e] = a[e];
+    r[e] = b[e];
+    if (w != nullptr && mine) {
+      p[e] *= inv * (double)w[ia + e];
+      r[e] *= inv * (double)w[ib + e];
+    }
+    if (turn != nullptr && mine) {
+      const double c = turn[e].x, s = turn[e].y, first = p[e] * c - r[e] * s;
+      r[e] = r[e] * c + p[e] * s;
+      p[e] = first;
+    }
+    big = max(big, max(__float_as_uint(__double2float_ru(fabs(p[e]))), __float_as_uint(__double2float_ru(fabs(r[e])))));
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(group, big, o));
+  Kv8Exact out;
+  out.e8 = kv8_exponent(big);
+  const double down = (double)__int_as_float((127 - out.e8) << 23);
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    out.codes[e / 4] = (unsigned)kv8_codes(kv8_odd(p[e] * down), kv8_odd(p[e + 1] * down)) |
+                       (unsigned)kv8_codes(kv8_odd(p[e + 2] * down), kv8_odd(p[e + 3] * down)) << 16;
+    out.codes[E / 4 + e / 4] = (unsigned)kv8_codes(kv8_odd(r[e] * down), kv8_odd(r[e + 1] * down)) |
+                               (unsigned)kv8_codes(kv8_odd(r[e + 2] * down), kv8_odd(r[e + 3] * down)) << 16;
+  }
+  return out;
+}
+
+template <int E> __device__ __forceinline__ void store_codes(unsigned char* dst, const unsigned* codes) {
+  if constexpr (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
+  else *reinterpret_cast<unsigned*>(dst) = codes[0];
+}
+
 // A group of LANES lanes (a power of two, at least D / 2E) takes a head's vector; a lane holds E pairs (a[i], b[i])
 // that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others pair up
 // (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 2E, so E pairs are two stretches of E elements.
 // E = 8 where rows and R allow 16-byte loads of bfloat16, else 4.  Queries are not measured for a scale, values not
-// normalised.  4,096 tokens of 32 + 16 heads of 128: 24.2 us, 0.60 of the copy peak, instructions issued in 72 % of the
-// cycles (34.6 us with E = 4); 64 tokens in 32 bits 3.2, one 2.5, most of it the launch and the first loads.
+// normalised.  4,096 tokens of 32 + 16 heads of 128: 27.5 us, 0.53 of the copy peak, instructions issued in most cycles
+// (34.6 with E = 4; 24.2 when keys' codes were those of 32-bit arithmetic: 1.7 for the span's second end, the rest for heads
+// taken again; with that inside the loop, where its registers count, 34.6).  64 tokens in 32 bits 5.0, one 3.4, most
+// of it the launch and the first loads.  Seven blocks an SM: 27.5 us, eight, with 40 bytes of spills, 28.3, six 28.5.
 template <typename T, int LANES, int E>
-__global__ void __launch_bounds__(128, 8)
+__global__ void __launch_bounds__(128, 7)
 kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__ q_out, int nq, const T* __restrict__ k,
                  long long k_stride, const T* __restrict__ v, long long v_stride, const float* __restrict__ q_weight,
                  const float* __restrict__ k_weight, float eps, const float2* __restrict__ table, int rot,
@@ -127,6 +201,7 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   fetch(head);
   // the first rows are on their way before the place is looked up
   const long long row = k == nullptr ? -1 : kv8_row(c, token_entry[token], positions[token], status, threadIdx.x == 0 && blockIdx.y == 0);
+  unsigned long long again = 0ull;               // key heads of this group to take again; the last bit stands for all after it
   for (; head < heads; head += warps * HEADS) {             // the same for a group's lanes
     const bool is_q = head < nq, is_k = !is_q && head < nq + c.nkv;
     float a[E], b[E];
@@ -171,27 +246,70 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
       big = max(big, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(group, big, o));
-    if (!mine || row < 0) continue;
+    if (row < 0) continue;
     const bool finite = big < 0x7f800000u;
     const int e8 = finite ? kv8_exponent(big) : 0;
     const float down = __int_as_float((127 - e8) << 23);
+    unsigned codes[E / 2];
+    // elements 0 .. E - 1 and E .. 2 E - 1 of the lane, each moved by `by` times the sum of its pair's magnitudes
+    auto encode = [&](auto moved, float by, unsigned (&to)[E / 2]) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        float x[4], y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = a[e + j] * down;
+          y[j] = b[e + j] * down;
+          if constexpr (decltype(moved)::value) {
+            const float at = (fabsf(x[j]) + fabsf(y[j])) * by;
+            x[j] += at;
+            y[j] += at;
+          }
+        }
+        to[e / 4] = (unsigned)kv8_codes(x[0], x[1]) | (unsigned)kv8_codes(x[2], x[3]) << 16;
+        to[E / 4 + e / 4] = (unsigned)kv8_codes(y[0], y[1]) | (unsigned)kv8_codes(y[2], y[3]) << 16;
+      }
+    };
+    if (is_k && finite && (w != nullptr || rot > 0)) {
+      // 32-bit errors in units of 2^-24: sum of squares 13 (two of a term, at most eleven sums) and the mean 2, half of it in
+      // the root, the root itself 4 (two ulp), weights 2, relative to an element; a rotation carries that over to
+      // a pair's length and adds at most 2 of it; and a pair's magnitudes sum to no less than its length
+      constexpr float SPAN = 16.f / 16777216.f;
+      unsigned other[E / 2];
+      encode(std::true_type(), -SPAN, codes);
+      encode(std::true_type(), SPAN, other);
+      bool apart = abs((int)(big & 0x7fffffu) - 0x600000) < 32;          // the scale's border
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) apart |= mine && codes[i] != other[i];
+      if (__any_sync(group, apart)) again |= 1ull << min((head - nq) / (warps * HEADS), 63);
+    } else if (finite) {
+      encode(std::false_type(), 0.f, codes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) codes[i] = 0u;
+    }
+    if (!mine) continue;
     const int kvh = is_k ? head - nq : head - nq - c.nkv;
     const size_t at = (size_t)row + (size_t)kvh * c.page_size;
     unsigned char* dst = (is_k ? c.k : c.v) + at * D;
-    unsigned codes[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      codes[e / 4] = !finite ? 0u : (unsigned)kv8_codes(a[e] * down, a[e + 1] * down) | (unsigned)kv8_codes(a[e + 2] * down, a[e + 3] * down) << 16;
-      codes[E / 4 + e / 4] = !finite ? 0u : (unsigned)kv8_codes(b[e] * down, b[e + 1] * down) | (unsigned)kv8_codes(b[e + 2] * down, b[e + 3] * down) << 16;
-    }
-    if constexpr (E == 8) {
-      *reinterpret_cast<uint2*>(dst + ia) = make_uint2(codes[0], codes[1]);
-      *reinterpret_cast<uint2*>(dst + ib) = make_uint2(codes[2], codes[3]);
-    } else {
-      *reinterpret_cast<unsigned*>(dst + ia) = codes[0];
-      *reinterpret_cast<unsigned*>(dst + ib) = codes[1];
-    }
+    store_codes<E>(dst + ia, codes);
+    store_codes<E>(dst + ib, codes + E / 4);
     if (l == 0) (is_k ? c.ks : c.vs)[at] = (unsigned char)(finite ? e8 + KV8_BIAS : KV8_NAN);
+  }
+  if (again == 0ull) return;
+  const int step = warps * HEADS;
+  int kvh = warp * HEADS + sub - nq;
+  if (kvh < 0) kvh += (-kvh + step - 1) / step * step;
+  for (; kvh < c.nkv; kvh += step) {
+    if (!(again >> min(kvh / step, 63) & 1ull)) continue;
+    const Kv8Exact sure = kv8_exact<T, LANES, E>(k_row + (size_t)kvh * D, k_weight, turns ? table + (size_t)token * half + pair : nullptr, ia, ib,
+                                                 mine, eps, D, group);
+    const size_t at = (size_t)row + (size_t)kvh * c.page_size;
+    if (mine) {
+      store_codes<E>(c.k + at * D + ia, sure.codes);
+      store_codes<E>(c.k + at * D + ib, sure.codes + E / 4);
+    }
+    if (l == 0) c.ks[at] = (unsigned char)(sure.e8 + KV8_BIAS);
   }
 }
 
