@@ -1999,7 +1999,9 @@ def kv8_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.T
     head are rotated in halves.  ``q`` [N, heads * D] of the same type goes the same way with ``q_norm`` and is
     stored in ``q_out`` [N, heads * D] (bfloat16, dense, not overlapping any input).
 
-    A position outside the block table or a missing page sets a bit of ``status`` and writes nothing."""
+    Codes and scales are those of exact arithmetic on what is given (keys' squares have to sum to a 32-bit number); the
+    queries are worked out in 32 bits.  A position outside the block table or a missing page sets a bit of ``status`` and
+    writes nothing."""
     num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
     some = q if k is None else k
     if (k is None) != (v is None) or (q is None) != (q_out is None) or some is None:
