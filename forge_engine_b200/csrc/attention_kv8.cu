@@ -641,11 +641,12 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   constexpr int UNIT = PORTION ? ROWS * WARPS : ROWS;
   pdl_trigger();
   pdl_wait();
-  const int kvh = blockIdx.x, slot = PORTION ? gridDim.y - 1 - blockIdx.y : blockIdx.y, piece = blockIdx.z;
-  int entry = slot, unit = 0;
+  const int kvh = blockIdx.x, piece = blockIdx.z;
+  int slot = blockIdx.y, entry = slot, unit = 0;
   if constexpr (PORTION) {
-    const Slot<UNIT> at(p, slot);
+    const Slot<UNIT, true> at(p, slot);
     if (at.entry < 0) return;
+    slot = at.slot;
     entry = at.entry;
     unit = at.unit;
   }

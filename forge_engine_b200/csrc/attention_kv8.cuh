@@ -75,20 +75,27 @@ __device__ __forceinline__ int key_page(const Kv8Attention& p, const int* table,
 
 // Which row tile of which entry a block takes: the tiles of UNIT rows of the entries with more than row_lo rows, one entry
 // after another; entry -1 past the last one.  A warp finds it, 32 entries at a time.  Entries that cannot be have one
-// tile, whose block says so.
-template <int UNIT> struct Slot {
-  int entry, unit;
-  __device__ __forceinline__ Slot(const Kv8Attention& p, int slot) : entry(-1), unit(0) {
+// tile, whose block says so.  FROM_LAST counts from the last tile, so that the tiles that see most keys come first and what
+// the grid has too many comes at its end.
+template <int UNIT, bool FROM_LAST> struct Slot {
+  int entry, unit, slot;
+  static __device__ __forceinline__ int units(const Kv8Attention& p, int e) {
+    if (e >= p.entries) return 0;
+    const long long rows = ((long long)p.cu_tokens[e + 1] - p.cu_tokens[e]) * p.groups;
+    const bool can_be = rows >= 0 && rows <= (long long)p.total_tokens * p.groups;
+    return !can_be ? 1 : rows > p.row_lo ? (int)((rows + UNIT - 1) / UNIT) : 0;
+  }
+  __device__ __forceinline__ Slot(const Kv8Attention& p, int index) : entry(-1), unit(0), slot(index) {
     const int lane = threadIdx.x & 31;
+    if constexpr (FROM_LAST) {
+      int all = 0;
+      for (int e0 = 0; e0 < p.entries; e0 += 32) all += __reduce_add_sync(0xffffffffu, units(p, e0 + lane));
+      slot = min(all, p.slots) - 1 - index;          // a grid that is too small takes the first ones
+      if (slot < 0) return;
+    }
     int before = 0;
     for (int e0 = 0; e0 < p.entries; e0 += 32) {
-      const int e = e0 + lane;
-      int mine = 0;
-      if (e < p.entries) {
-        const long long rows = ((long long)p.cu_tokens[e + 1] - p.cu_tokens[e]) * p.groups;
-        const bool can_be = rows >= 0 && rows <= (long long)p.total_tokens * p.groups;
-        mine = !can_be ? 1 : rows > p.row_lo ? (int)((rows + UNIT - 1) / UNIT) : 0;
-      }
+      const int mine = units(p, e0 + lane);
       int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -223,11 +230,11 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
 constexpr int JOIN_ROWS = D <= 64 ? 32 : D <= 128 ? 16 : 8;         // eight columns of a row a thread
 template <int UNIT, int TILE>
 __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention p) {
-  constexpr int BLOCKS = UNIT / JOIN_ROWS, STRETCHES = D / 8, BATCH = 8;
+  constexpr int BLOCKS = UNIT / JOIN_ROWS, STRETCHES = D / 8, BATCH = 4;
   pdl_trigger();
   pdl_wait();
   const int slot = blockIdx.x / BLOCKS, kvh = blockIdx.y;
-  const Slot<UNIT> at(p, slot);
+  const Slot<UNIT, false> at(p, slot);
   if (at.entry < 0) return;
   const Entry e(p, at.entry);
   const int rows = e.n_new * p.groups, row0 = at.unit * UNIT, r0 = (blockIdx.x - slot * BLOCKS) * JOIN_ROWS;

@@ -202,9 +202,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   pdl_trigger();
   pdl_wait();
   // blocks start in the order of x, y, z: the row tiles that see most keys first
-  const int kvh = blockIdx.x, slot = gridDim.y - 1 - blockIdx.y, piece = blockIdx.z;
-  const Slot<PORTION_UNIT> at(p, slot);
+  const int kvh = blockIdx.x, piece = blockIdx.y;
+  const Slot<PORTION_UNIT, true> at(p, blockIdx.z);
   if (at.entry < 0) return;
+  const int slot = at.slot;
   const Entry e(p, at.entry);
   const int rows = e.n_new * p.groups, row0 = at.unit * PORTION_UNIT;
   if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
@@ -677,7 +678,7 @@ int launch_portion(Kv8Attention p, cudaStream_t stream) {
   p.ws_rows = PORTION_UNIT;
   const cudaError_t err = cudaFuncSetAttribute(attn_kv8_portion_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
   if (err != cudaSuccess) return (int)err;
-  int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)p.slots, (unsigned)p.spans), dim3(THREADS), SMEM, stream, p);
+  int rc = fe_launch_dependent(attn_kv8_portion_kernel, dim3((unsigned)p.nkv, (unsigned)p.spans, (unsigned)p.slots), dim3(THREADS), SMEM, stream, p);
   if (rc == 0 && p.spans > 1)
     rc = launch_join_portion<PORTION_UNIT, PORTION_TILE>(p, stream);
   return rc;
