@@ -39,11 +39,11 @@ _NOTHING = _Nothing()
 class BuildContext:
     """What every part may know about its surroundings."""
 
-    dtype: object  # torch.float32 or torch.bfloat16: dtype of activations and of the KV cache
+    dtype: object  # torch.float32 or torch.bfloat16: dtype of activations, and of a KV cache that is not in 8 bits
     device: object
     status: object  # int32[1] device word kernels set error bits in
-    cache_dtype: str | None = None  # "float8": layers that can keep their keys and values in 8 bits do
     timer: object = None  # None, or an object whose ``section(name)`` brackets a part's call with events
+    cache_dtype: str | None = None  # "float8": layers that can keep their keys and values in 8 bits do
 
     def section(self, name: str):
         """A context manager round one part's work: records events when a timer is set."""
@@ -76,10 +76,10 @@ class CacheView:
     owns: bool
     state: object = None
     own_state: object = None
-    # (scales of the keys, of the values) [pages, kv_heads, page_size] where ``kv`` is an 8-bit cache
-    scales: tuple | None = None
     # further states of the run by name (``CacheNeeds.states``), each [max_requests + 1, *shape]
     states: dict = field(default_factory=dict)
+    # (scales of the keys, of the values) [pages, kv_heads, page_size] where ``kv`` is an 8-bit cache
+    scales: tuple | None = None
 
 
 class Part:

@@ -71,3 +71,15 @@ def test_settings() -> None:
     for needs in ([eight, wide], [None], [CacheNeeds()]):
         with pytest.raises(ConfigError):
             check_cache(needs, "float8")
+
+
+def test_parts_are_built_and_views_made_by_position_as_before() -> None:
+    """What the 8-bit cache added to the parts' interfaces comes after what was there."""
+    from forge_engine_b200.parts.base import BuildContext, CacheView
+
+    timer, status = object(), object()
+    ctx = BuildContext(torch.bfloat16, "cpu", status, timer)
+    assert ctx.timer is timer and ctx.status is status and ctx.cache_dtype is None
+    state, own, states = object(), object(), {"a": 1}
+    view = CacheView(None, 0, True, state, own, states)
+    assert view.state is state and view.own_state is own and view.states is states and view.scales is None
