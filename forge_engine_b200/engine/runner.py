@@ -40,7 +40,7 @@ def check_cache(needs: list, cache_dtype: str | None) -> None:
     for run, kv in paged:
         if not kv.eight_bit:
             raise ConfigError(f"cache_dtype='float8': the layer of run {run} has no form over an 8-bit cache (plain grouped-query "
-                              "attention of the bfloat16 engine has one, with a window and a rotation of whole multiples of 8)")
+                              "attention of the bfloat16 engine has one, with a positive scale, a window and a rotation of whole multiples of 8)")
 
 
 def resolve_dtype(name) -> torch.dtype:

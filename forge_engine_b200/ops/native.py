@@ -1903,6 +1903,11 @@ def kv8_takes(head_dim: int) -> bool:
     return head_dim % 16 == 0 and 16 <= head_dim <= 256
 
 
+def kv8_takes_scale(scale: float) -> bool:
+    """Whether the attention over the 8-bit cache takes this factor of the scores: positive and not beyond 32-bit numbers."""
+    return 0.0 < scale <= 3.4028234663852886e38
+
+
 def kv8_lib(head_dim: int):
     """The attention over the 8-bit cache compiled for ``head_dim`` (built on first use): (call, workspace size)."""
     got = _kv8_handles.get(head_dim)
@@ -2167,8 +2172,8 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     q_stride = _kv8_rows(q, n, num_q_heads * d, "q")
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape:
         raise UnsupportedShapeError("q and out are bfloat16 of one shape")
-    if n_entries < 0 or max_new < 0 or window < 0 or keep_first < 0 or not scale > 0:
-        raise UnsupportedShapeError("attention_kv8: no negative sizes, and a positive scale")
+    if n_entries < 0 or max_new < 0 or window < 0 or keep_first < 0 or not kv8_takes_scale(scale):
+        raise UnsupportedShapeError("attention_kv8: no negative sizes, and a positive, finite scale")
     if (cu_tokens.dtype != torch.int32 or starts.dtype != torch.int32 or cu_tokens.numel() <= n_entries or starts.numel() < n_entries
             or block_table.shape[0] < n_entries):
         raise UnsupportedShapeError("cu_tokens holds entries + 1 int32 numbers, starts one an entry, block_table a row")

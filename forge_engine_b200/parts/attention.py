@@ -241,15 +241,20 @@ class GQAttention(Mixer):
                            and self.chunk is None and self.keep_first == 0 and self.softcap is None and self.query_temperature is None
                            and self.slopes is None and self.distance_bias is None and self.sinks is None
                            and not self.head_gate and not self.output_gate)
-        # keys and values in 8 bits: a plain layer of the bfloat16 engine, rotated (if at all) by a table of angles
-        rotary = self.position.rotary()
-        self.eight_bit = (ctx.cache_dtype == "float8" and not self.general and ctx.dtype == torch.bfloat16 and native.kv8_takes(self.d)
-                          and (rotary is None or (hasattr(self.position, "table") and rotary[1] % 8 == 0)))
+        self.eight_bit = ctx.cache_dtype == "float8" and self._has_eight_bit_form()
         self._slots = None
         self.plan_key = ("gqa_attention", self.nq, self.nkv, self.d, spec.window) + (
             ("general", self.dv, self.parts, self.keep_first, self.chunk) if self.general and not self.plain_core else ()) + (
             ("float8",) if self.eight_bit else ())
         self.last_splits = None   # what the last step's decode entries ran with (0: balanced kernel)
+
+    def _has_eight_bit_form(self) -> bool:
+        """Whether the layer can keep keys and values in 8 bits: a plain layer of the bfloat16 engine whose scores are multiplied
+        by a positive number, rotated (if at all) by a table of angles."""
+        if self.general or self.ctx.dtype != torch.bfloat16 or not native.kv8_takes(self.d) or not native.kv8_takes_scale(self.spec.scale):
+            return False
+        rotary = self.position.rotary()
+        return rotary is None or (hasattr(self.position, "table") and rotary[1] % 8 == 0)
 
     @staticmethod
     def _o_bias(spec) -> bool:

@@ -134,3 +134,9 @@ def test_plans_take_any_pairs_once() -> None:
     assert native.kv8_plan(((700, 1), (3, 40)), 32, 8, 128, None, 0) == want
     # a context that grows by a token at a time changes its plan at most four times while it doubles
     assert len({native.kv8_plan([(n, 1)], 32, 8, 128) for n in range(4096, 8192)}) <= 5
+
+
+@pytest.mark.parametrize("scale", [float("inf"), 1e39])
+def test_attention_refuses_scales_beyond_32_bits(scale) -> None:
+    with pytest.raises(UnsupportedShapeError):
+        native.attention_kv8(**attention_args(scale=scale))

@@ -83,3 +83,32 @@ def test_parts_are_built_and_views_made_by_position_as_before() -> None:
     state, own, states = object(), object(), {"a": 1}
     view = CacheView(None, 0, True, state, own, states)
     assert view.state is state and view.own_state is own and view.states is states and view.scales is None
+
+
+def attention_layer(scale: float, position=None, cache_dtype="float8", dtype=torch.bfloat16):
+    from forge_engine_b200.config.specs import AttentionSpec, NoPositionSpec
+    from forge_engine_b200.parts.attention import GQAttention
+    from forge_engine_b200.parts.base import BuildContext
+
+    spec = AttentionSpec(32, 4, 2, 16, False, 1e-6, False, scale, position or NoPositionSpec(), None)
+    weights = {name: torch.zeros(info.shape, dtype=dtype) for name, info in GQAttention.weight_shapes(spec).items()}
+    return GQAttention(spec, weights, BuildContext(dtype, torch.device("cpu"), None, cache_dtype=cache_dtype))
+
+
+def test_layers_whose_scale_the_kernels_refuse_are_refused_at_build() -> None:
+    """A layer that multiplies its scores by nothing positive runs over a wide cache alone: the model says so when it is
+    built, not in its first step."""
+    for scale, takes in ((0.25, True), (1.0, True), (0.0, False), (-0.25, False), (float("inf"), False), (float("nan"), False)):
+        layer = attention_layer(scale)
+        assert layer.eight_bit == takes and layer.cache_needs().kv.eight_bit == takes
+        if not takes:
+            with pytest.raises(ConfigError):
+                check_cache([layer.cache_needs()], "float8")
+    assert not attention_layer(0.25, dtype=torch.float32).eight_bit and not attention_layer(0.25, cache_dtype=None).eight_bit
+
+
+def test_a_layer_over_a_wide_cache_does_not_ask_its_position_encoding_when_built(monkeypatch) -> None:
+    from forge_engine_b200.parts.base import PositionEncoding
+
+    monkeypatch.setattr(PositionEncoding, "rotary", lambda self: pytest.fail("asked"))
+    assert not attention_layer(0.25, cache_dtype=None).eight_bit
