@@ -1894,6 +1894,7 @@ KV8_FEW_ROWS, KV8_SINGLE_ROWS = 8, 16     # rows (new tokens x heads per kv head
 KV8_TILE = 128               # keys of a tile
 KV8_POSITIONS = 0x7fff0000   # a sequence's positions are below
 KV8_TC5_DIMS = (64, 128)     # head sizes whose portions the tcgen05 kernel takes
+KV8_MOST_UNITS = 65535       # row tiles of portions that a call takes: an axis of a grid
 
 _kv8_handles: dict = {}
 
@@ -2083,7 +2084,9 @@ def kv8_plan(entries, num_q_heads: int, num_kv_heads: int, head_dim: int, window
     if not portion:
         return (*few_cut, *single_cut, 1, 0, 0)
     cut = _kv8_cut(portion, num_kv_heads, *(_KV8_PORTION if tc5 else _KV8_PORTION_MMA))
-    return (*few_cut, *single_cut, *cut, _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, len(portion))])
+    units = _KV8_SPANS[_bisect.bisect_left(_KV8_SPANS, len(portion))]
+    # rounding up must not carry a call that the kernels take beyond what they take
+    return (*few_cut, *single_cut, *cut, min(units, max(KV8_MOST_UNITS, len(portion))))
 
 
 def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, tile: int) -> int:

@@ -140,3 +140,10 @@ def test_plans_take_any_pairs_once() -> None:
 def test_attention_refuses_scales_beyond_32_bits(scale) -> None:
     with pytest.raises(UnsupportedShapeError):
         native.attention_kv8(**attention_args(scale=scale))
+
+
+@pytest.mark.parametrize("tiles", [49152, 49153, 60000, 65535, 65536])
+def test_row_tiles_are_rounded_within_what_a_call_takes(tiles) -> None:
+    """A plan's count of row tiles is rounded up, but not beyond what the kernels take while the true count is within it."""
+    units = native.kv8_plan([(0, 4 * tiles)], 16, 1, 96, 128)[6]
+    assert units >= tiles and (units <= 65535) == (tiles <= 65535)
