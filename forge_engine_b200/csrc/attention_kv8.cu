@@ -107,10 +107,11 @@ struct Queries {
       for (int i = 0; i < D / 4; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const bool finite = big < 0x7f800000u;                     // a row that is not gives NaN, also where every score is minus infinity
       int e2 = (int)(big >> 23) - 127 - 14;                      // 2^e2 is taken out of the row
-      e2 = big == 0u || big >= 0x7f800000u ? 0 : max(e2, -100);
+      e2 = big == 0u || !finite ? 0 : max(e2, -100);
       const float down = __int_as_float((127 - e2) << 23);
-      factor[h] = p.scale_log2 * __int_as_float((127 + e2) << 23);
+      factor[h] = finite ? p.scale_log2 * __int_as_float((127 + e2) << 23) : kv8_scale(KV8_NAN);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         a[s][h] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);

@@ -32,3 +32,30 @@ def test_small_scales_and_queries_of_zeros(native, dim, scale) -> None:  # noqa:
         out, status = attend(native, cache, requests, q, window, keep, scale)
         assert status == 0
         check_attention(cache, requests, q, out, window, keep, scale)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("dim,requests", [(128, [(90, 1), (20, 2)]), (128, [(90, 4), (5, 3)]), (96, [(90, 1), (50, 4)]), (96, [(90, 30)]),
+                                          (48, [(90, 1), (50, 4), (20, 30)]), (64, [(90, 30)])])
+def test_queries_that_are_infinite_give_nan(native, dim, requests, value) -> None:  # noqa: F811
+    """An infinite element of a query makes its head's output NaN, also where every score is minus infinity; no other
+    row notices."""
+    heads, nkv, page = 8, 2, 16
+    g = torch.Generator().manual_seed(dim)
+    values = []
+    for s, n in requests:
+        k, v = (torch.randn((s + n, nkv, dim), generator=g, dtype=torch.float64) for _ in range(2))
+        k[:, :, 5] = -math.copysign(1.0, value) * (1 + k[:, :, 5].abs())
+        values.append((k, v))
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5, values=values)
+    q = rows_of(requests, heads, dim, 4)
+    bad = torch.zeros((q.shape[0], heads), dtype=torch.bool)
+    at = 0
+    for _, n in requests:
+        bad[at, 1] = bad[at + n - 1, heads - 1] = True
+        at += n
+    q.view(-1, heads, dim)[:, :, 5][bad] = value
+    for plan in (None, (1, 2, 1, 2, 1, 2, 8)):
+        out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, plan=plan)
+        got = out[:at].view(at, heads, dim)
+        assert status == 0 and bool(torch.isnan(got[bad[:at]]).all()) and bool(torch.isfinite(got[~bad[:at]]).all())
