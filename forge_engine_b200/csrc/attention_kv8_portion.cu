@@ -497,9 +497,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
           unsigned char* part = q_tiles + x * 2 * CODE_TILE + code_offset(at, c >> 1) + (c & 1) * 8;
           *reinterpret_cast<uint2*>(part) = make_uint2(__byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
           *reinterpret_cast<uint2*>(part + CODE_TILE) = make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
-          // what a score is multiplied by, in log2 units, goes to the lane whose row it is.  Never zero, because masked scores,
-          // minus infinity by then, are multiplied too: products are below 2^90, so what a factor of 2^-126 leaves is nothing
-          const float up = finite ? fmaxf(p.scale_log2 * __int_as_float((127 + ex) << 23), 1.17549435e-38f) : kv8_scale(KV8_NAN);
+          // what a score is multiplied by, in log2 units, goes to the lane whose row it is
+          const float up = finite ? p.scale_log2 * __int_as_float((127 + ex) << 23) : kv8_scale(KV8_NAN);
           const float got = __shfl_sync(0xffffffffu, up, (lane % Q_ROWS) * Q_LANES);
           if (lane / Q_ROWS == n0 + n) factor = got;
         }
@@ -507,6 +506,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive(q_full + x);
+      // Never zero, because masked scores, minus infinity by then, are multiplied too: products are below 2^90, so what a
+      // factor of 2^-126 leaves is nothing.
+      if (factor < 0x1p-126f) factor = 0x1p-126f;
     }
     float m = -INFINITY, l = 0.f;
     bool ok = mine.valid;
