@@ -11,13 +11,15 @@
 // exponent, u_j = t_j + b_j.  The running maximum M is that of u_j, the largest contribution to the output, so
 // the weights 2^(u_j - M) of the value product lie in [0, 1] whatever the scales are, and the codes go into the
 // tensor cores as the half-precision numbers they exactly are (one conversion instruction for two codes).  The
-// denominator sums 2^(t_j - M) = 2^(u_j - M) 2^(-b_j) in 32 bits.  Weights are rounded to half precision (11
+// denominator sums 2^(t_j - M) = 2^(u_j - M) 2^(-b_j) in 32 bits (small scales: see denominator_term).  Weights are rounded to half precision (11
 // bits; what is below 2^-25 of the largest contribution vanishes).  A query row is scaled by a power of two so
 // that its largest element lies in [2^14, 2^15): bfloat16's 8 bits stay whole down to 2^-31 of that.
 //
 // Upstream's counterparts read pages of the model's type: the eager attention of
 // src/forge_engine/qwen3.py:187-206 and the decode kernel of src/forge_engine/kernels/cuda_paged.py:276-347.
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "attention_kv8.cuh"
 
@@ -56,6 +58,19 @@ __device__ __forceinline__ float exp2_fast(float x) {       // the weight is rou
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// What a key adds to the sum that divides: 2^(t - M) = w 2^(-b), with w = 2^(u - M) at hand and `back` 2^(-b).  But w is zero below
+// 2^-126, and a value of zeros, whose b is the least, beside one with a b of 63 would not count at all.  So a warp that
+// met a scale below 2^-32 walks its keys once more with SMALL, where that exponential is taken by itself and `back` is b.
+// (Above it w vanishes only where t is 30 below that of the largest contribution, whose M is at most that t + 64.)
+constexpr int SMALL_SCALE = KV8_BIAS - 32;
+template <bool SMALL> __device__ __forceinline__ float denominator_term(float u, float base, float w, float back, float sum) {
+  return SMALL ? sum + exp2_fast(u - base - back) : fmaf(w, back, sum);
+}
+// What sums with maximum `from` are worth with maximum `to`.  With SMALL the root of it: a sum may then be 2^64 of its weights
+// and the maxima of keys that count alike 2^128 apart, so it goes its way in two halves.
+template <bool SMALL> __device__ __forceinline__ float worth(float from, float to) {
+  return from == -INFINITY ? 0.f : exp2f(SMALL ? 0.5f * (from - to) : from - to);
 }
 __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -187,6 +202,7 @@ __device__ __forceinline__ int value_column(int n, int c, int t) {
 }
 
 // The 32 keys of a stage, at positions from key0 on, against a warp's 16 rows.
+template <bool SMALL>
 __device__ __forceinline__ void take(const Queries& q, const unsigned char* stage, int key0, const Kv8Attention& p, bool clear,
                                      int pos_a, int pos_b, Sums& s, int lane) {
   const int g = lane >> 2, t = lane & 3;
@@ -238,24 +254,27 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
     const float now = fmaxf(s.m[h], mx[h]);
-    corr[h] = s.m[h] == -INFINITY ? 0.f : exp2f(s.m[h] - now);
+    corr[h] = worth<SMALL>(s.m[h], now);
     s.m[h] = now;
     base[h] = now == -INFINITY ? 0.f : now;
   }
   if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+    const float by[2] = {SMALL ? corr[0] * corr[0] : corr[0], SMALL ? corr[1] * corr[1] : corr[1]};
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) { s.o[n][0] *= corr[0]; s.o[n][1] *= corr[0]; s.o[n][2] *= corr[1]; s.o[n][3] *= corr[1]; }
+    for (int n = 0; n < D / 8; ++n) { s.o[n][0] *= by[0]; s.o[n][1] *= by[0]; s.o[n][2] *= by[1]; s.o[n][3] *= by[1]; }
   }
 #pragma unroll
   for (int k = 0; k < STEP / 16; ++k) {
     unsigned a[4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const float2 back = make_float2(of_key[16 * k + 8 * n + 2 * t].z, of_key[16 * k + 8 * n + 2 * t + 1].z);
+      const float4 k0 = of_key[16 * k + 8 * n + 2 * t], k1 = of_key[16 * k + 8 * n + 2 * t + 1];
+      const float2 back = make_float2(SMALL ? k0.y : k0.z, SMALL ? k1.y : k1.z);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float w0 = exp2_fast(c[2 * k + n][2 * h] - base[h]), w1 = exp2_fast(c[2 * k + n][2 * h + 1] - base[h]);
-        sum[h] = fmaf(w0, back.x, fmaf(w1, back.y, sum[h]));
+        const float u0 = c[2 * k + n][2 * h], u1 = c[2 * k + n][2 * h + 1];
+        const float w0 = exp2_fast(u0 - base[h]), w1 = exp2_fast(u1 - base[h]);
+        sum[h] = denominator_term<SMALL>(u0, base[h], w0, back.x, denominator_term<SMALL>(u1, base[h], w1, back.y, sum[h]));
         a[2 * n + h] = pack_half(w0, w1);
       }
     }
@@ -267,7 +286,7 @@ __device__ __forceinline__ void take(const Queries& q, const unsigned char* stag
     if constexpr (D > 16 && (D & 16) != 0) value_stretch<D / 32 * 32, 2>(vs, 16 * k, a, s.o, lane);
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) s.l[h] = s.l[h] * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
+  for (int h = 0; h < 2; ++h) s.l[h] = (SMALL ? s.l[h] * corr[h] : s.l[h]) * corr[h] + sum[h];       // this lane's keys; the quad's sums join at the end
 }
 
 // The codes of a step's 32 keys and values; lane l knows the row of key l in its cache (-1: none, zeros).  ALL: every key
@@ -311,13 +330,16 @@ struct WarpRing {
   const Kv8Attention& p;
   const int* table;
   int kvh, key_lo, key_end, lane, page, k_scale, v_scale;
+  int least_scale;                 // of the lane's values so far
   __device__ __forceinline__ WarpRing(unsigned char* ring, const Kv8Attention& p, const int* table, int kvh, int key_lo, int key_end, int lane)
-      : ring(ring), p(p), table(table), kvh(kvh), key_lo(key_lo), key_end(key_end), lane(lane), page(-1), k_scale(KV8_BIAS), v_scale(KV8_BIAS) {}
+      : ring(ring), p(p), table(table), kvh(kvh), key_lo(key_lo), key_end(key_end), lane(lane), page(-1), k_scale(KV8_BIAS), v_scale(KV8_BIAS),
+        least_scale(KV8_BIAS) {}
   __device__ __forceinline__ unsigned char* stage(int i) const { return ring + (i & 1) * STAGE; }
   __device__ __forceinline__ void look_up(int key0) { page = key_page(p, table, key0 + lane, key_end); }
   // The scales of step i, asked for with its codes.  A key whose value is not finite counts as not finite itself.
-  __device__ __forceinline__ void put_scales(int i) const {
+  __device__ __forceinline__ void put_scales(int i) {
     const bool bad = v_scale == KV8_NAN;
+    least_scale = min(least_scale, v_scale);
     reinterpret_cast<float4*>(stage(i) + 2 * MATRIX)[lane] =
         make_float4(kv8_scale(bad ? KV8_NAN : k_scale), bad ? 0.f : (float)(v_scale - KV8_BIAS),
                     bad ? 1.f : __int_as_float((2 * KV8_BIAS - v_scale) << 23), 0.f);
@@ -436,6 +458,7 @@ __device__ __forceinline__ void row_values(const unsigned char* vs, int k0, cons
 }
 
 // The 32 keys of a stage against eight rows.
+template <bool SMALL>
 __device__ __forceinline__ void take_rows(const RowQueries& q, const unsigned char* stage, int key0, const Kv8Attention& p, bool clear,
                                           const int (&pos)[2], RowSums& s, int lane) {
   const int g = lane >> 2, t = lane & 3;
@@ -470,7 +493,7 @@ __device__ __forceinline__ void take_rows(const RowQueries& q, const unsigned ch
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float4 of = of_key[16 * j + 8 * h + g];
-      back[j][h] = of.z;
+      back[j][h] = SMALL ? of.y : of.z;
       const int key = key0 + 16 * j + 8 * h + g;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -490,15 +513,16 @@ __device__ __forceinline__ void take_rows(const RowQueries& q, const unsigned ch
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
     const float now = fmaxf(s.m[i], mx[i]);
-    corr[i] = s.m[i] == -INFINITY ? 0.f : exp2f(s.m[i] - now);
+    corr[i] = worth<SMALL>(s.m[i], now);
     s.m[i] = now;
     base[i] = now == -INFINITY ? 0.f : now;
   }
   if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-    s.l[0] *= corr[0];
-    s.l[1] *= corr[1];
+    const float by[2] = {SMALL ? corr[0] * corr[0] : corr[0], SMALL ? corr[1] * corr[1] : corr[1]};
+    s.l[0] = (SMALL ? s.l[0] * corr[0] : s.l[0]) * corr[0];
+    s.l[1] = (SMALL ? s.l[1] * corr[1] : s.l[1]) * corr[1];
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) { s.o[d][0] *= corr[0]; s.o[d][1] *= corr[1]; s.o[d][2] *= corr[0]; s.o[d][3] *= corr[1]; }
+    for (int d = 0; d < D / 16; ++d) { s.o[d][0] *= by[0]; s.o[d][1] *= by[1]; s.o[d][2] *= by[0]; s.o[d][3] *= by[1]; }
   }
   const unsigned char* vs = stage + MATRIX;
 #pragma unroll
@@ -507,8 +531,8 @@ __device__ __forceinline__ void take_rows(const RowQueries& q, const unsigned ch
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float w0 = exp2_fast(u[j][2 * h] - base[0]), w1 = exp2_fast(u[j][2 * h + 1] - base[1]);
-      s.l[0] = fmaf(w0, back[j][h], s.l[0]);
-      s.l[1] = fmaf(w1, back[j][h], s.l[1]);
+      s.l[0] = denominator_term<SMALL>(u[j][2 * h], base[0], w0, back[j][h], s.l[0]);
+      s.l[1] = denominator_term<SMALL>(u[j][2 * h + 1], base[1], w1, back[j][h], s.l[1]);
       b[h] = transposed(pack_half(w0, w1));
     }
     row_values<0, D >= 128 ? 16 : D >= 64 ? 8 : 4>(vs, 16 * j, b, s, lane);
@@ -543,10 +567,10 @@ __device__ __forceinline__ void finish_rows(const Kv8Attention& p, const Entry& 
     float den = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = piece_share(ml[(w * ROWS + r) * 2], ml[(w * ROWS + r) * 2 + 1], big);
+      const float l = ml[(w * ROWS + r) * 2 + 1], root = piece_share_root(ml[(w * ROWS + r) * 2], l, big), f = root * root;
       const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROWS + r) * D + d);
       num.x += x.x * f; num.y += x.y * f; num.z += x.z * f; num.w += x.w * f;
-      den += ml[(w * ROWS + r) * 2 + 1] * f;
+      den += l * root * root;
     }
     if (pieces == 1) {
       const float inv = den == 0.f ? 0.f : 1.f / den;
@@ -578,36 +602,41 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kerne
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   auto key0_of = [&](int i) -> int { return walk.tile(begin + i) * KEYS + warp * STEP; };
   WarpRing mine(smem + warp * (STAGES * STAGE), p, p.block_table + (size_t)entry * p.max_pages, kvh, walk.key_lo, walk.key_end, lane);
-  mine.look_up(key0_of(0));
   RowQueries q;
   RowSums s;
   int pos[2];                        // rows past the end take the last row's position; nobody reads them
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    pos[i] = e.start + min(2 * t + i, rows - 1) / p.groups;
-    s.m[i] = -INFINITY;
-    s.l[i] = 0.f;
-  }
+  for (int i = 0; i < 2; ++i) pos[i] = e.start + min(2 * t + i, rows - 1) / p.groups;
+  auto walk_keys = [&](auto small) {
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) { s.o[d][0] = s.o[d][1] = s.o[d][2] = s.o[d][3] = 0.f; }
+    for (int i = 0; i < 2; ++i) {
+      s.m[i] = -INFINITY;
+      s.l[i] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) { s.o[d][0] = s.o[d][1] = s.o[d][2] = s.o[d][3] = 0.f; }
+    mine.look_up(key0_of(0));
 #pragma unroll 1
-  for (int i = -1; i < steps; ++i) {
-    if (i >= 0) mine.put_scales(i);
-    if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
-    cp_async_commit();
-    if (i < 0) {
-      q.load(p, e, kvh, rows, lane);
-      continue;
+    for (int i = -1; i < steps; ++i) {
+      if (i >= 0) mine.put_scales(i);
+      if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
+      cp_async_commit();
+      if (i < 0) {
+        q.load(p, e, kvh, rows, lane);
+        continue;
+      }
+      cp_async_wait<1>();
+      __syncwarp();
+      const int key0 = key0_of(i);
+      if (key0 <= walk.pos_last) {
+        const bool clear = key0 + STEP - 1 <= walk.pos_first && (p.window <= 0 || walk.pos_last - key0 < p.window);
+        take_rows<decltype(small)::value>(q, mine.stage(i), key0, p, clear, pos, s, lane);
+      }
+      __syncwarp();
     }
-    cp_async_wait<1>();
-    __syncwarp();
-    const int key0 = key0_of(i);
-    if (key0 <= walk.pos_last) {
-      const bool clear = key0 + STEP - 1 <= walk.pos_first && (p.window <= 0 || walk.pos_last - key0 < p.window);
-      take_rows(q, mine.stage(i), key0, p, clear, pos, s, lane);
-    }
-    __syncwarp();
-  }
+  };
+  walk_keys(std::false_type());
+  if (__any_sync(0xffffffffu, mine.least_scale < SMALL_SCALE)) walk_keys(std::true_type());
   __syncthreads();                   // the rings' space takes the warps' sums
   float* acc = reinterpret_cast<float*>(smem);           // [WARPS][16][D]
   float* ml = acc + WARPS * ROWS * D;                    // [WARPS][16][2]
@@ -673,27 +702,31 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   const int pos_min = e.start + min(wrow0, last) / p.groups, pos_max = e.start + min(wrow0 + ROWS - 1, last) / p.groups;
   Queries q;
   Sums s;
-  s.clear();
   WarpRing mine(ring, p, table, kvh, walk.key_lo, walk.key_end, lane);
-  mine.look_up(key0_of(0));
+  auto walk_keys = [&](auto small) {
+    s.clear();
+    mine.look_up(key0_of(0));
 #pragma unroll 1
-  for (int i = -1; i < steps; ++i) {
-    if (i >= 0) mine.put_scales(i);
-    if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
-    cp_async_commit();
-    if (i < 0) {
-      q.load(p, e, kvh, wrow0, rows_end, lane);
-      continue;
+    for (int i = -1; i < steps; ++i) {
+      if (i >= 0) mine.put_scales(i);
+      if (i + 1 < steps) mine.ask(i + 1, key0_of(i + 1), i + 2 < steps ? key0_of(i + 2) : walk.key_end);
+      cp_async_commit();
+      if (i < 0) {
+        q.load(p, e, kvh, wrow0, rows_end, lane);
+        continue;
+      }
+      cp_async_wait<1>();
+      __syncwarp();
+      const int key0 = key0_of(i);
+      if (key0 <= pos_max) {
+        const bool clear = key0 + STEP - 1 <= pos_min && (p.window <= 0 || pos_max - key0 < p.window);
+        take<decltype(small)::value>(q, ring + (i & 1) * STAGE, key0, p, clear, pos_a, pos_b, s, lane);
+      }
+      __syncwarp();
     }
-    cp_async_wait<1>();
-    __syncwarp();
-    const int key0 = key0_of(i);
-    if (key0 <= pos_max) {
-      const bool clear = key0 + STEP - 1 <= pos_min && (p.window <= 0 || pos_max - key0 < p.window);
-      take(q, ring + (i & 1) * STAGE, key0, p, clear, pos_a, pos_b, s, lane);
-    }
-    __syncwarp();
-  }
+  };
+  walk_keys(std::false_type());
+  if (__any_sync(0xffffffffu, mine.least_scale < SMALL_SCALE)) walk_keys(std::true_type());
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);

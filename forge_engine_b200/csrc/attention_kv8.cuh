@@ -132,10 +132,11 @@ __device__ __forceinline__ void store_row(const Kv8Attention& p, const Entry& e,
   p.out[((size_t)(e.tok0 + token) * p.nkv * p.groups + kvh * p.groups + g) * D + d] = __float2bfloat16_rn(v);
 }
 
-// The share of a piece with maximum m and sum l in a join whose largest maximum is `big`.  A piece that saw no
-// key has no part; one whose every score was NaN has no maximum, but its sum says so.
-__device__ __forceinline__ float piece_share(float m, float l, float big) {
-  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - big);
+// The root of the share of a piece with maximum m and sum l in a join whose largest maximum is `big`.  A piece that saw no
+// key has no part; one whose every score was NaN has no maximum, but its sum says so.  (Where M is that of u = t + b, a sum may
+// be 2^64 of its weights and the maxima of keys that count alike 2^128 apart: sums go their way in two halves.)
+__device__ __forceinline__ float piece_share_root(float m, float l, float big) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(0.5f * (m - big));
 }
 
 // Element (row r of the unit, column d) of a piece's sums: stretches of eight columns, the rows' stretches side by
@@ -184,8 +185,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_kv8_join_kernel(Kv8Atten
     float share = 0.f;
     if (k0 + lane < mine) {
       const float* at = ml + (size_t)(warp + (k0 + lane) * JOIN_WARPS) * step;
-      share = piece_share(at[0], at[1], big);
-      den += at[1] * share;
+      const float root = piece_share_root(at[0], at[1], big);
+      share = root * root;
+      den += at[1] * root * root;
     }
     const int here = min(32, mine - k0);
 #pragma unroll 8
@@ -268,15 +270,15 @@ __global__ void __launch_bounds__(256) attn_kv8_join_portion_kernel(Kv8Attention
     }
 #pragma unroll
     for (int s = 0; s < BATCH; ++s) now = fmaxf(now, of[s].x);
-    const float corr = big == -INFINITY ? 1.f : exp2f(big - now);         // what is there without a maximum is 0 or NaN
-    den *= corr;
+    const float root = big == -INFINITY ? 1.f : exp2f(0.5f * (big - now));         // what is there without a maximum is 0 or NaN
+    den = den * root * root;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) num[c] *= corr;
+    for (int c = 0; c < 8; ++c) num[c] *= root * root;
     big = now;
 #pragma unroll
     for (int s = 0; s < BATCH; ++s) {
-      const float share = piece_share(of[s].x, of[s].y, big);
-      den += of[s].y * share;
+      const float root = piece_share_root(of[s].x, of[s].y, big), share = root * root;
+      den += of[s].y * root * root;
       num[0] += a[s].x * share; num[1] += a[s].y * share; num[2] += a[s].z * share; num[3] += a[s].w * share;
       num[4] += b[s].x * share; num[5] += b[s].y * share; num[6] += b[s].z * share; num[7] += b[s].w * share;
     }

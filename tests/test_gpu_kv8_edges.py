@@ -59,3 +59,32 @@ def test_queries_that_are_infinite_give_nan(native, dim, requests, value) -> Non
         out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, plan=plan)
         got = out[:at].view(at, heads, dim)
         assert status == 0 and bool(torch.isnan(got[bad[:at]]).all()) and bool(torch.isfinite(got[~bad[:at]]).all())
+
+
+def zero_values(which: str, length: int) -> torch.Tensor:
+    """Which of a request's values are zero."""
+    at = torch.arange(length)
+    return {"every other": at % 2 == 0, "first half": at < length // 2, "second half": at >= length // 2, "all but one": at != length // 3}[which]
+
+
+@pytest.mark.parametrize("which", ["every other", "first half", "second half", "all but one"])
+@pytest.mark.parametrize("dim,requests", [(128, [(900, 1), (333, 2)]), (128, [(700, 4)]), (48, [(700, 1), (200, 4)]), (96, [(700, 60)]),
+                                          (128, [(700, 60)])])
+def test_zeros_beside_the_largest_values_count(native, dim, requests, which) -> None:  # noqa: F811
+    """Values of zeros, whose scale is the least there is, beside values whose scale is near the largest: each key counts in
+    the sum that divides, whatever its value's scale."""
+    heads, nkv, page = 8, 2, 16
+    g = torch.Generator().manual_seed(dim)
+    values = []
+    for s, n in requests:
+        k, v = (torch.randn((s + n, nkv, dim), generator=g, dtype=torch.float64) for _ in range(2))
+        v *= 2.0 ** 70
+        v[zero_values(which, s + n)] = 0
+        values.append((k, v))
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5, values=values)
+    assert {int(x) for x in cache["v_scale"].view(torch.uint8).unique()} >= {63} and int(cache["v_scale"].view(torch.uint8)[cache["v_scale"].view(torch.uint8) < 255].max()) >= 190
+    q = rows_of(requests, heads, dim, 4)
+    for plan in (None, (1, 16, 1, 16, 1, 16, 8), (100, 1, 100, 1, 100, 1, 8)):
+        out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, plan=plan)
+        assert status == 0
+        check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
