@@ -145,6 +145,8 @@ template <int E> __device__ __forceinline__ void store_codes(unsigned char* dst,
   else *reinterpret_cast<unsigned*>(dst) = codes[0];
 }
 
+constexpr int WRITE_ROUNDS = 64;                 // heads a group of lanes takes one after the other, at most
+
 // A group of LANES lanes (a power of two, at least D / 2E) takes a head's vector; a lane holds E pairs (a[i], b[i])
 // that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others pair up
 // (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 2E, so E pairs are two stretches of E elements.
@@ -201,7 +203,7 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   fetch(head);
   // the first rows are on their way before the place is looked up
   const long long row = k == nullptr ? -1 : kv8_row(c, token_entry[token], positions[token], status, threadIdx.x == 0 && blockIdx.y == 0);
-  unsigned long long again = 0ull;               // key heads of this group to take again; the last bit stands for all after it
+  unsigned long long again = 0ull;               // key heads of this group to take again, by rounds: there are at most WRITE_ROUNDS
   for (; head < heads; head += warps * HEADS) {             // the same for a group's lanes
     const bool is_q = head < nq, is_k = !is_q && head < nq + c.nkv;
     float a[E], b[E];
@@ -281,7 +283,7 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
       bool apart = abs((int)(big & 0x7fffffu) - 0x600000) < 32;          // the scale's border
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) apart |= mine && codes[i] != other[i];
-      if (__any_sync(group, apart)) again |= 1ull << min((head - nq) / (warps * HEADS), 63);
+      if (__any_sync(group, apart)) again |= 1ull << (head - nq) / (warps * HEADS);
     } else if (finite) {
       encode(std::false_type(), 0.f, codes);
     } else {
@@ -301,7 +303,7 @@ kv8_write_kernel(const T* __restrict__ q, long long q_stride, bf16* __restrict__
   int kvh = warp * HEADS + sub - nq;
   if (kvh < 0) kvh += (-kvh + step - 1) / step * step;
   for (; kvh < c.nkv; kvh += step) {
-    if (!(again >> min(kvh / step, 63) & 1ull)) continue;
+    if (!(again >> kvh / step & 1ull)) continue;
     const Kv8Exact sure = kv8_exact<T, LANES, E>(k_row + (size_t)kvh * D, k_weight, turns ? table + (size_t)token * half + pair : nullptr, ia, ib,
                                                  mine, eps, D, group);
     const size_t at = (size_t)row + (size_t)kvh * c.page_size;
@@ -383,6 +385,8 @@ int kv8_write_typed(const void* q, long long q_stride, bf16* q_out, int nq, cons
   const int rounds = (heads + 4 * heads_a_warp - 1) / (4 * heads_a_warp);      // of a block of four warps over a token's heads
   // few tokens: blocks share a token's heads until the chip has about two blocks an SM
   int share = rounds < (296 + tokens - 1) / tokens ? rounds : (296 + tokens - 1) / tokens;
+  if (share < (rounds + WRITE_ROUNDS - 1) / WRITE_ROUNDS) share = (rounds + WRITE_ROUNDS - 1) / WRITE_ROUNDS;
+  if (share > 65535) return FE_ERR_TOO_LARGE;
   const dim3 grid((unsigned)tokens, (unsigned)share);
   auto launch = [&](auto kernel) {
     return fe_launch_dependent(kernel, grid, dim3(128), 0, stream, (const T*)q, q_stride, q_out, nq, (const T*)k, k_stride,

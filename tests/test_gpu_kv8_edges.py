@@ -88,3 +88,33 @@ def test_zeros_beside_the_largest_values_count(native, dim, requests, which) -> 
         out, status = attend(native, cache, requests, q, 0, 0, dim ** -0.5, plan=plan)
         assert status == 0
         check_attention(cache, requests, q, out, 0, 0, dim ** -0.5)
+
+
+@pytest.mark.parametrize("rot", [8, 16])
+def test_hundreds_of_heads_some_not_finite(native, rot) -> None:  # noqa: F811
+    """More heads than a writing warp has rounds to note which it takes again: keys that are not finite stay so."""
+    dim, nkv, page, tokens = 256, 1200, 16, 300
+    g = torch.Generator().manual_seed(rot)
+    row = torch.randn((1, nkv * dim), generator=g)
+    bad = [0, 5, 300, 511, 700, 902, 1100, 1199]
+    for i, head in enumerate(bad):
+        row[0, head * dim + (37 * i) % dim] = (math.inf, -math.inf, math.nan)[i % 3]
+    angle = torch.rand((1, rot // 2), generator=g).double()
+    table = torch.stack((angle.cos(), angle.sin()), -1).float()
+    pages = -(-tokens // page)
+    caches = empty_caches(pages, nkv, page, dim)
+    status = status_word()
+    rows = row.to(DEV).expand(tokens, -1)
+    native.kv8_write(rows, rows, ints(range(tokens)), ints([0] * tokens), *caches, ints(range(pages)).view(1, pages), status,
+                     table=table.expand(tokens, -1, -1).contiguous().to(DEV))
+    assert int(status.item()) == 0
+    heads = row.view(1, nkv, dim)
+    finite = torch.where(torch.isfinite(heads).all(-1, keepdim=True), heads, torch.full_like(heads, math.nan))
+    for x, codes, scales in ((plain.norm_rotate(finite, None, 0.0, table), caches[0], caches[2]), (heads.double(), caches[1], caches[3])):
+        want_codes, want_scales = plain.quantise(x[0])
+        got_scales = scales.view(torch.uint8).transpose(1, 2).reshape(pages * page, nkv)[:tokens]
+        got_codes = codes.view(torch.uint8).transpose(1, 2).reshape(pages * page, nkv, dim)[:tokens]
+        assert torch.equal(got_scales, want_scales.to(DEV).expand(tokens, -1))
+        want = want_codes.float().to(plain.CODES).view(torch.uint8).to(DEV)
+        # a zero has two signs
+        assert bool(((got_codes == want) | (((got_codes | want) & 0x7F) == 0)).all())
