@@ -330,7 +330,7 @@ struct WarpRing {
   const Kv8Attention& p;
   const int* table;
   int kvh, key_lo, key_end, lane, page, k_scale, v_scale;
-  int least_scale;                 // of the lane's values so far
+  int least_scale;                   // of the lane's values so far
   __device__ __forceinline__ WarpRing(unsigned char* ring, const Kv8Attention& p, const int* table, int kvh, int key_lo, int key_end, int lane)
       : ring(ring), p(p), table(table), kvh(kvh), key_lo(key_lo), key_end(key_end), lane(lane), page(-1), k_scale(KV8_BIAS), v_scale(KV8_BIAS),
         least_scale(KV8_BIAS) {}

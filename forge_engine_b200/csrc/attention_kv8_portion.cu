@@ -427,7 +427,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
         if (ok && more) tc5::umma_commit(freed + ((i + 1) & 3));
       }
       tc5::umma_commit(o_full + x);
+      // a role that gave up: what was issued is over before tensor memory is given back
+      for (unsigned n = 0; !ok && n < WAIT_TRIES && !tc5::mbar_try_wait(o_full + x, 0); ++n) {}
     }
+    __syncwarp();          // the warp is whole again before barriers and tensor memory
   } else {
     // ---- softmax: a thread a row of query tile x ----
     const int x = warp >> 2;
@@ -618,6 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
       ++count;
       ++commits;
     }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");       // of weights of a step that was given up
     if (ok) ok = __all_sync(0xffffffffu, wait(o_full + x, 0, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
