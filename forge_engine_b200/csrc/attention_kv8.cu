@@ -594,7 +594,10 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1) attn_kv8_rows_kerne
   const int kvh = blockIdx.x, entry = blockIdx.y, piece = blockIdx.z;
   const Entry e(p, entry);
   const int rows = e.n_new * p.groups;
-  if (rows <= p.row_lo || rows > p.row_hi) return;
+  if (rows <= p.row_lo || rows > p.row_hi) {
+    if (kvh == 0 && piece == 0 && threadIdx.x == 0 && left_out(p, rows)) atomicOr(p.status, FE_STATUS_LEFT_OUT);
+    return;
+  }
   const Walk<KEYS> walk(p, e.start, 0, rows);
   const int pieces = pieces_of(p, walk.count);
   if (piece >= pieces) return;
@@ -682,7 +685,10 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_mma_kernel(Kv8Attention p) {
   }
   const Entry e(p, entry);
   const int rows = e.n_new * p.groups, row0 = unit * UNIT;
-  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) return;
+  if (rows <= p.row_lo || rows > p.row_hi || row0 < 0 || row0 >= rows) {
+    if (!PORTION && kvh == 0 && piece == 0 && threadIdx.x == 0 && left_out(p, rows)) atomicOr(p.status, FE_STATUS_LEFT_OUT);
+    return;
+  }
   const int rows_end = min(rows, row0 + UNIT);
   const Walk<KEYS> walk(p, e.start, row0, rows_end);
   const int pieces = pieces_of(p, walk.count);
@@ -839,14 +845,15 @@ FE_EXPORT long long SYM(fe_attention_kv8_workspace_d)(int entries, int max_new, 
 }
 
 // The entries of a step with at most 8 rows (new tokens x heads per kv head) if few_spans is above zero, those with 9 to 16
-// if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.  The portions' row tiles number at
-// most portion_units.
+// if single_spans is, the others if portion_spans is; `*_span` key tiles of 128 a block, `*_spans` of them for the longest.  The
+// portions' row tiles number at most portion_units.  Entries and row tiles that this leaves out set a status bit, unless there
+// are fillers, entries whose rows nobody reads.
 FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* out, const void* k, const void* v, const void* ks,
                                       const void* vs, const int* block_table, int max_pages, int page_size, int num_pages,
                                       int nkv, int groups, const int* cu_tokens, const int* starts, int entries, int max_new, int total_tokens,
                                       int window, int keep_first, float scale, int few_span, int few_spans,
                                       int single_span, int single_spans, int portion_units, int portion_span, int portion_spans,
-                                      float* workspace, int* status,
+                                      int fillers, float* workspace, int* status,
                                       cudaStream_t stream) {
   if (entries <= 0 || max_new <= 0 || total_tokens <= 0) return 0;
   if (page_size < 1 || nkv < 1 || groups < 1 || window < 0 || keep_first < 0 || keep_first > 0x7fff0000 || max_pages < 0 || num_pages < 0) return FE_ERR_BAD_SHAPE;
@@ -867,6 +874,9 @@ FE_EXPORT int SYM(fe_attention_kv8_d)(const void* q, long long q_stride, void* o
   p.entries = entries; p.max_new = max_new; p.slots = 0; p.ws_rows = 0;
   p.window = window; p.keep_first = keep_first; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.ws = workspace;
+  // a plan without anything still finds out whether there are rows
+  if (!fillers && few_spans == 0 && single_spans == 0 && portion_spans == 0) few_spans = 1;
+  p.kinds = fillers ? KINDS_ALL_TOLD : (few_spans > 0 ? 1 : 0) | (single_spans > 0 ? 2 : 0) | (portion_spans > 0 ? 4 : 0);
   if (few_spans > 0) {
     p.row_lo = 0; p.row_hi = 8; p.span = few_span; p.spans = few_spans;
     const int rc = launch_single(p, stream);

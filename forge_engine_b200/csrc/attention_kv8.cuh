@@ -13,6 +13,8 @@ namespace kv8 {
 constexpr int D = FE_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 up to 256");
 
+constexpr int KINDS_ALL_TOLD = 15;          // of Kv8Attention::kinds: what a launch leaves out is nobody's
+
 struct Kv8Attention {
   const bf16* q;
   long long q_stride;
@@ -30,6 +32,7 @@ struct Kv8Attention {
   int entries, max_new;    // max_new: the most tokens an entry has
   int slots;               // single tokens: entries; portions: row tiles of all of them (see Slot)
   int ws_rows;             // rows of a unit, at most; even
+  int kinds;               // bit 0, 1, 2: entries of up to 8, up to 16, more rows are launched (see left_out)
   float* ws;               // [slots, nkv, spans][ws_rows x (D + 2)]: see piece_element
 };
 
@@ -67,6 +70,11 @@ struct Entry {
   }
 };
 
+// An entry with rows of a kind that the call's plan has not got would be left as it was: somebody who meets it says so.
+__device__ __forceinline__ bool left_out(const Kv8Attention& p, long long rows) {
+  return rows > 0 && !(p.kinds >> (rows <= 8 ? 0 : rows <= 16 ? 1 : 2) & 1);
+}
+
 // The page of a key, or -1 where it is missing; asked for a tile before the key is, so that nothing waits for it.
 __device__ __forceinline__ int key_page(const Kv8Attention& p, const int* table, int key, int key_end) {
   const int logical = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
@@ -79,23 +87,34 @@ __device__ __forceinline__ int key_page(const Kv8Attention& p, const int* table,
 // the grid has too many comes at its end.
 template <int UNIT, bool FROM_LAST> struct Slot {
   int entry, unit, slot;
-  static __device__ __forceinline__ int units(const Kv8Attention& p, int e) {
-    if (e >= p.entries) return 0;
-    const long long rows = ((long long)p.cu_tokens[e + 1] - p.cu_tokens[e]) * p.groups;
+  static __device__ __forceinline__ long long rows_of(const Kv8Attention& p, int e) {
+    return e < p.entries ? ((long long)p.cu_tokens[e + 1] - p.cu_tokens[e]) * p.groups : 0;
+  }
+  static __device__ __forceinline__ int units(const Kv8Attention& p, long long rows) {
     const bool can_be = rows >= 0 && rows <= (long long)p.total_tokens * p.groups;
     return !can_be ? 1 : rows > p.row_lo ? (int)((rows + UNIT - 1) / UNIT) : 0;
+  }
+  // every block of the grid finds it, one says it
+  static __device__ __forceinline__ void tell(const Kv8Attention& p) {
+    if (p.kinds != KINDS_ALL_TOLD && blockIdx.x + blockIdx.y + blockIdx.z == 0) atomicOr(p.status, FE_STATUS_LEFT_OUT);
   }
   __device__ __forceinline__ Slot(const Kv8Attention& p, int index) : entry(-1), unit(0), slot(index) {
     const int lane = threadIdx.x & 31;
     if constexpr (FROM_LAST) {
       int all = 0;
-      for (int e0 = 0; e0 < p.entries; e0 += 32) all += __reduce_add_sync(0xffffffffu, units(p, e0 + lane));
+      bool left = false;
+      for (int e0 = 0; e0 < p.entries; e0 += 32) {
+        const long long rows = rows_of(p, e0 + lane);
+        left |= left_out(p, rows);
+        all += __reduce_add_sync(0xffffffffu, units(p, rows));
+      }
+      if (left || all > p.slots) tell(p);
       slot = min(all, p.slots) - 1 - index;          // a grid that is too small takes the first ones
       if (slot < 0) return;
     }
     int before = 0;
     for (int e0 = 0; e0 < p.entries; e0 += 32) {
-      const int mine = units(p, e0 + lane);
+      const int mine = units(p, rows_of(p, e0 + lane));
       int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

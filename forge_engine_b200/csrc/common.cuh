@@ -26,6 +26,8 @@
 #define FE_STATUS_BAD_PAGE 2       // block table entry outside the pool or negative
 #define FE_STATUS_BAD_POSITION 4   // position outside the block table
 #define FE_STATUS_WAIT_TIMEOUT 8   // a bounded wait inside a kernel ran out
+// 16: the sampling kernels' bit for logits that are not finite (sampling.cu)
+#define FE_STATUS_LEFT_OUT 32      // an entry is not in the plan of the attention call that should take it
 
 #define FE_EXPORT extern "C" __attribute__((visibility("default")))
 

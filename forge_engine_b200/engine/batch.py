@@ -57,6 +57,7 @@ class StepBatch:
     # ``plan_step`` of the model); filled before a step is captured in a CUDA graph, so that
     # the replayed kernels are the ones the step's real entries call for.
     plans: dict = field(default_factory=dict)
+    fillers: bool = False      # whether there are entries whose rows nobody reads (see ``plan_batch``)
 
 
 @dataclass
@@ -72,6 +73,7 @@ class BatchPlan:
     entries: list          # (slot, start, count) per entry
     max_new: int
     max_ctx: int
+    fillers: bool = False
 
 
 def plan_batch(entries: Sequence[StepEntry], cache, *, pad_counts: Sequence[int] = (), table_width: int | None = None,
@@ -156,7 +158,7 @@ def plan_batch(entries: Sequence[StepEntry], cache, *, pad_counts: Sequence[int]
     for g, (_, rows) in enumerate(tables):
         put(f"table{g}", rows)
     return BatchPlan(flat, offsets, n, r, len(want_rows), [w for w, _ in tables], host,
-                     max([c for _, _, c in host] + list(pad_counts), default=1), max(ctx_lens))
+                     max([c for _, _, c in host] + list(pad_counts), default=1), max(ctx_lens), pad_entries > 0)
 
 
 def batch_from_buffer(plan: BatchPlan, device_buffer: torch.Tensor) -> StepBatch:
@@ -182,6 +184,7 @@ def batch_from_buffer(plan: BatchPlan, device_buffer: torch.Tensor) -> StepBatch
         entries=plan.entries,
         max_new=plan.max_new,
         max_ctx=plan.max_ctx,
+        fillers=plan.fillers,
     )
 
 

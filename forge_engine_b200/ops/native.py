@@ -26,6 +26,7 @@ STATUS_BITS = {
     4: "a position lies outside its request's block table",
     8: "a bounded wait inside a kernel ran out",
     16: "logits contain NaN or +inf",
+    32: "an entry of an attention call is not in the call's plan",
 }
 
 _ERRORS = {
@@ -1920,7 +1921,7 @@ def kv8_lib(head_dim: int):
             raise CUDAUnavailableError(f"cannot load {path}: {error}") from error
         p, i, f, ll = c_void_p, c_int, c_float, ctypes.c_longlong
         fn, size = getattr(handle, f"fe_attention_kv8_d{head_dim}"), getattr(handle, f"fe_attention_kv8_workspace_d{head_dim}")
-        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, i, i, i, p, p, p]
+        fn.argtypes = [p, ll, p, p, p, p, p, p, i, i, i, i, i, p, p, i, i, i, i, i, f, i, i, i, i, i, i, i, i, p, p, p]
         fn.restype = c_int
         size.argtypes = [i, i, i, i, i, i, i, i]
         size.restype = ll
@@ -2160,14 +2161,17 @@ def _kv8_cut(tiles: list, nkv: int, slots: int, alone: float, full: float, block
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                   block_table: torch.Tensor, cu_tokens: torch.Tensor, starts: torch.Tensor, n_entries: int, max_new: int,
                   num_q_heads: int, window: int | None, keep_first: int, scale: float, out: torch.Tensor, status: torch.Tensor,
-                  plan: tuple) -> None:
+                  plan: tuple, *, fillers: bool = False) -> None:
     """Causal grouped-query attention over an 8-bit cache (``kv8_write``), which holds the new tokens already.
 
     ``q`` [N, heads * D] (bfloat16; rows any multiple of four elements apart) are the queries of ``n_entries`` entries:
     entry e's are rows ``cu_tokens[e]`` .. ``cu_tokens[e + 1]``, at positions ``starts[e]`` on (``cu_tokens``, ``starts``
     int32 on the device; at most ``max_new`` rows an entry).  A query sees every key up to its own, or with ``window``
     the last ``window`` of them and the first ``keep_first`` of the sequence.  ``out`` [N, heads * D] (bfloat16, dense); rows
-    of no entry are left as they are.  ``plan``: ``kv8_plan`` of these entries.  32-bit scores, softmax and sums."""
+    of no entry are left as they are.  ``plan``: ``kv8_plan`` of these entries.  An entry of a kind that the plan has
+    not got (up to 8 rows, up to 16, more) and row tiles beyond those that it counted set a bit of ``status``, and their rows are
+    left as they are; with ``fillers`` - entries beside the planned ones, there for a fixed size, whose rows nobody reads -
+    without the bit.  32-bit scores, softmax and sums."""
     num_pages, nkv, page_size, d = _kv8_caches(k_cache, v_cache, k_scale, v_scale, block_table, status)
     window, keep_first, n = window or 0, keep_first or 0, q.shape[0]
     if num_q_heads < 1 or num_q_heads % nkv:
@@ -2197,4 +2201,4 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               (q.data_ptr(), q_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                block_table.data_ptr(), block_table.shape[1], page_size, num_pages, nkv, groups, cu_tokens.data_ptr(),
                starts.data_ptr(), n_entries, max_new, n, window, keep_first, scale, few_span, few_spans, single_span, single_spans, portion_units,
-               portion_span, portion_spans, ptr(workspace), status.data_ptr()), "attention_kv8")
+               portion_span, portion_spans, int(fillers), ptr(workspace), status.data_ptr()), "attention_kv8")

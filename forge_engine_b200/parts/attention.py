@@ -395,7 +395,8 @@ class GQAttention(Mixer):
         out = torch.empty_like(q)
         with self.ctx.section("mixer.attention"):
             native.attention_kv8(q, *caches, table, batch.cu_tokens, batch.starts, batch.n_entries, batch.max_new, self.nq,
-                                 self.spec.window, 0, self.spec.scale, out, self.ctx.status, batch.plans[self.plan_key])
+                                 self.spec.window, 0, self.spec.scale, out, self.ctx.status, batch.plans[self.plan_key],
+                                 fillers=batch.fillers)
         return out
 
     def _attend_general(self, x, batch, cache: CacheView):

@@ -118,3 +118,75 @@ def test_hundreds_of_heads_some_not_finite(native, rot) -> None:  # noqa: F811
         want = want_codes.float().to(plain.CODES).view(torch.uint8).to(DEV)
         # a zero has two signs
         assert bool(((got_codes == want) | (((got_codes | want) & 0x7F) == 0)).all())
+
+
+KINDS = {"few": [(300, 1), (40, 2)], "single": [(300, 4), (17, 3)], "portion": [(260, 70), (5, 30)]}
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96, 48])
+@pytest.mark.parametrize("planned", [("few",), ("single",), ("portion",), ("few", "portion"), ("single", "portion"), ("few", "single"), ()])
+def test_entries_outside_the_plan_are_told(native, dim, planned) -> None:  # noqa: F811
+    """An entry of a kind that the plan has not got sets the status bit and is left as it was; the others are right.  With
+    fillers the same without the bit."""
+    heads, nkv, page = 8, 2, 16
+    requests = [r for pair in zip(*KINDS.values()) for r in pair]
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5)
+    caches = tuple(cache[name].view(torch.uint8).to(DEV).view(cache[name].dtype) for name in ("k_cache", "v_cache", "k_scale", "v_scale"))
+    q = rows_of(requests, heads, dim, 4)
+    inside = [r for kind in planned for r in KINDS[kind]]
+    ends = [0]
+    for _, n in requests:
+        ends.append(ends[-1] + n)
+    made = native.kv8_plan(inside, heads, nkv, dim)
+    for plan in (made, *(tuple(2 if i in (0, 2, 4) else 2 * (made[i] > 0) if i in (1, 3, 5) else made[i] for i in range(7)) for _ in made[1::2])):
+        for fillers in (False, True):
+            out, status = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV), status_word()
+            native.attention_kv8(q.to(DEV), *caches, cache["table"].to(DEV), ints(ends), ints(s for s, _ in requests), len(requests), 70, heads,
+                                 None, 0, dim ** -0.5, out, status, plan, fillers=fillers)
+            assert int(status.item()) == (0 if fillers else 32)
+            for e, request in enumerate(requests):
+                rows = out[ends[e] : ends[e + 1]].cpu()
+                if request in inside:
+                    one = {**cache, "held": [cache["held"][e]]}
+                    check_attention(one, [request], q[ends[e] : ends[e + 1]], rows, 0, 0, dim ** -0.5)
+                elif planned or fillers or request not in KINDS["few"]:
+                    assert bool((rows == 7.0).all()), request
+
+
+@pytest.mark.parametrize("dim", [64, 96])
+@pytest.mark.parametrize("spans", [1, 3])
+def test_row_tiles_beyond_the_plan_are_told(native, dim, spans) -> None:  # noqa: F811
+    """A plan with fewer row tiles than the entries have: the first ones are right, nothing else is written, and the status
+    says so - unless the others are fillers."""
+    heads, nkv, page, requests = 8, 2, 16, [(100, 70), (0, 300), (30, 90)]
+    rows_of_tile = 256 if dim == 64 else 64
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, 5)
+    caches = tuple(cache[name].view(torch.uint8).to(DEV).view(cache[name].dtype) for name in ("k_cache", "v_cache", "k_scale", "v_scale"))
+    q = rows_of(requests, heads, dim, 4)
+    ends = [0, 70, 370, 460]
+    tiles = [-(-n * heads // nkv // rows_of_tile) for _, n in requests]
+    first = tiles[0] + tiles[1]
+    for units, bit in ((first, 32), (tiles[0] + 1, 32), (sum(tiles), 0), (sum(tiles) + 5, 0)):
+        for fillers in (False, True):
+            out, status = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV), status_word()
+            native.attention_kv8(q.to(DEV), *caches, cache["table"].to(DEV), ints(ends), ints(s for s, _ in requests), 3, 300, heads, None, 0,
+                                 dim ** -0.5, out, status, (1, 0, 1, 0, 1 if spans > 1 else 100, spans, units), fillers=fillers)
+            assert int(status.item()) == (0 if fillers else bit)
+            out = out.cpu()
+            whole = sum(1 for i in range(3) if sum(tiles[: i + 1]) <= units)
+            check_attention({**cache, "held": cache["held"][:whole]}, requests[:whole], q, out, 0, 0, dim ** -0.5)
+            # of the entry that is cut off, the tokens of the tiles that are there
+            written = ends[whole] + (units - sum(tiles[:whole])) * rows_of_tile * nkv // heads if whole < 3 else 460
+            assert bool((out[written:] == 7.0).all())
+
+
+def test_more_tokens_than_said_are_told_by_a_plan_of_portions(native) -> None:  # noqa: F811
+    """``max_new`` says that there is no portion, the plan that there is nothing else: nothing fits, and the status says so."""
+    dim, heads, nkv, page = 64, 8, 2, 16
+    cache = plain.pool([300], nkv, dim, page, 1)
+    caches = tuple(cache[name].view(torch.uint8).to(DEV).view(cache[name].dtype) for name in ("k_cache", "v_cache", "k_scale", "v_scale"))
+    q = rows_of([(0, 40)], heads, dim, 2).to(DEV)
+    out, status = torch.full_like(q, 7.0), status_word()
+    native.attention_kv8(q, *caches, cache["table"].to(DEV), ints([0, 40]), ints([260]), 1, 3, heads, None, 0, 1.0, out, status,
+                         native.kv8_plan([(260, 40)], heads, nkv, dim))
+    assert int(status.item()) == 4 and bool((out == 7.0).all())
