@@ -190,3 +190,56 @@ def test_more_tokens_than_said_are_told_by_a_plan_of_portions(native) -> None:  
     native.attention_kv8(q, *caches, cache["table"].to(DEV), ints([0, 40]), ints([260]), 1, 3, heads, None, 0, 1.0, out, status,
                          native.kv8_plan([(260, 40)], heads, nkv, dim))
     assert int(status.item()) == 4 and bool((out == 7.0).all())
+
+
+# head sizes above 128 that are not 256: stretches of 128 and what is left of 64, 32 and 16 columns
+LARGE_DIMS = [144, 160, 176, 192, 208, 224, 240]
+
+
+@pytest.mark.parametrize("dim", LARGE_DIMS)
+def test_head_sizes_between_128_and_256(native, dim) -> None:  # noqa: F811
+    """Few rows, 9 to 16 rows and portions, uncut and cut, with and without a window."""
+    heads, nkv, page, requests = 8, 2, 16, [(300, 1), (150, 2), (260, 4), (31, 3), (140, 40), (0, 70), (0, 1)]
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, dim)
+    q = rows_of(requests, heads, dim, 3)
+    for plan in (None, (1, 4, 1, 4, 1, 4, 12), (2, 2, 2, 2, 2, 2, 12), (100, 1, 100, 1, 100, 1, 12)):
+        for window, keep in ((0, 0), (70, 20)):
+            out, status = attend(native, cache, requests, q, window, keep, dim ** -0.5, plan=plan)
+            assert status == 0
+            check_attention(cache, requests, q, out, window, keep, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", LARGE_DIMS)
+def test_writing_and_reading_head_sizes_between_128_and_256(native, dim, dtype) -> None:  # noqa: F811
+    """Norm, partial rotation, codes, scales and the way back; keys and values alone take the exact codes."""
+    tokens, nq, nkv, page, eps = 37, 3, 2, 16, 2.0 ** -20
+    for rot in (dim, 24, 0):
+        g = torch.Generator().manual_seed(dim + rot)
+        x = (torch.randn((tokens, (nq + 2 * nkv) * dim), generator=g) * 2).to(dtype)
+        weights = [torch.exp(0.3 * torch.randn(dim, generator=g)) for _ in range(2)] if rot else [None, None]
+        table = None
+        if rot:
+            angle = torch.rand((tokens, rot // 2), generator=g).double() * 2 * math.pi
+            table = torch.stack((angle.cos(), angle.sin()), -1).float()
+        pages = -(-tokens // page)
+        caches = empty_caches(pages, nkv, page, dim)
+        status, table_of = status_word(), ints(range(pages)).view(1, pages)
+        places = ints(range(tokens)), ints([0] * tokens)
+        q, k, v = x.to(DEV).split((nq * dim, nkv * dim, nkv * dim), dim=1)
+        q_out = torch.empty((tokens, nq * dim), dtype=torch.bfloat16, device=DEV)
+        on = [None if w is None else w.to(DEV) for w in weights]
+        native.kv8_write(k, v, *places, *caches, table_of, status, q=q, q_out=q_out, q_norm=on[0], k_norm=on[1], eps=eps,
+                         table=None if table is None else table.to(DEV))
+        outs = [torch.empty((tokens, nkv, dim), dtype=torch.float32, device=DEV) for _ in range(2)]
+        native.kv8_read(*caches, table_of, *places, *outs, status)
+        assert int(status.item()) == 0
+        split = x.double().view(tokens, nq + 2 * nkv, dim)
+        want_q = plain.norm_rotate(split[:, :nq], weights[0], eps, table)
+        size = want_q.abs().amax(-1, keepdim=True)
+        got_q = q_out.cpu().double().view(tokens, nq, dim)
+        # rounding to bfloat16 once; 32-bit norm and rotation before it are off by less than 2^-18 of the pair
+        assert bool(((got_q - want_q).abs() <= 2.0 ** -8 * want_q.abs() + 2.0 ** -18 * size).all())
+        for want, got in ((plain.norm_rotate(split[:, nq : nq + nkv], weights[1], eps, table), outs[0]), (split[:, nq + nkv :], outs[1])):
+            codes, scales = plain.quantise(want)
+            assert torch.equal(got.cpu().double(), codes * torch.exp2(scales.double() - 127)[..., None])
