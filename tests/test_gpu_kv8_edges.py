@@ -243,3 +243,59 @@ def test_writing_and_reading_head_sizes_between_128_and_256(native, dim, dtype) 
         for want, got in ((plain.norm_rotate(split[:, nq : nq + nkv], weights[1], eps, table), outs[0]), (split[:, nq + nkv :], outs[1])):
             codes, scales = plain.quantise(want)
             assert torch.equal(got.cpu().double(), codes * torch.exp2(scales.double() - 127)[..., None])
+
+
+@pytest.mark.parametrize("dim,requests", [(64, [(500, 1), (333, 70), (7, 200)]), (128, [(77, 3), (500, 90), (0, 33)])])
+@pytest.mark.parametrize("page", [1, 5, 48])
+@pytest.mark.parametrize("window,keep", [(0, 0), (130, 9)])
+def test_pages_of_any_size_and_queries_inside_wider_rows(native, dim, requests, page, window, keep) -> None:  # noqa: F811
+    """Pages that end inside a key tile, and queries that are columns of a projection, eight bytes from where 16 would be."""
+    heads, nkv = 8, 2
+    cache = plain.pool([s + n for s, n in requests], nkv, dim, page, dim + page)
+    q = rows_of(requests, heads, dim, 3)
+    wide = torch.full((q.shape[0], heads * dim + 24), 9.0, dtype=torch.bfloat16)
+    wide[:, 4 : 4 + heads * dim] = q
+    caches = tuple(cache[name].view(torch.uint8).to(DEV).view(cache[name].dtype) for name in ("k_cache", "v_cache", "k_scale", "v_scale"))
+    ends = [0]
+    for _, n in requests:
+        ends.append(ends[-1] + n)
+    for plan in (native.kv8_plan(requests, heads, nkv, dim, window, keep), (1, 3, 1, 3, 2, 3, 12)):
+        out, status = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV), status_word()
+        native.attention_kv8(wide.to(DEV)[:, 4 : 4 + heads * dim], *caches, cache["table"].to(DEV), ints(ends), ints(s for s, _ in requests),
+                             len(requests), max(n for _, n in requests), heads, window, keep, dim ** -0.5, out, status, plan)
+        assert int(status.item()) == 0 and bool((out[ends[-1] :] == 7.0).all())
+        check_attention(cache, requests, q, out.cpu(), window, keep, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim,nkv", [(128, 8), (256, 4), (48, 8)])
+def test_caches_past_32_bit_offsets(native, dim, nkv) -> None:  # noqa: F811
+    """Pages that lie more than 2^32 bytes into a cache, beside pages at its start: written, read back and attended."""
+    heads, page = 2 * nkv, 64
+    pages = 2 ** 32 // (nkv * page * dim) + 100
+    codes = [torch.empty((pages, nkv, page, dim), dtype=torch.uint8, device=DEV).view(plain.CODES) for _ in range(2)]
+    scales = [torch.empty((pages, nkv, page), dtype=torch.uint8, device=DEV).view(plain.SCALES) for _ in range(2)]
+    caches = (*codes, *scales)
+    requests = [(150, 1), (100, 60)]
+    table = ints([pages - 1, 0, pages - 7, pages - 2, 3, pages - 50]).view(2, 3)
+    g = torch.Generator().manual_seed(dim)
+    held = []
+    status = status_word()
+    for e, (s, n) in enumerate(requests):
+        x = torch.randn((s + n, 2 * nkv * dim), generator=g)
+        k, v = x.to(DEV).split((nkv * dim, nkv * dim), dim=1)
+        places = ints(range(s + n)), ints([e] * (s + n))
+        native.kv8_write(k, v, *places, *caches, table, status)
+        outs = [torch.empty((s + n, nkv, dim), device=DEV) for _ in range(2)]
+        native.kv8_read(*caches, table, *places, *outs, status)
+        both = []
+        for t, out in zip(x.view(s + n, 2 * nkv, dim).split((nkv, nkv), dim=1), outs):
+            c, b = plain.quantise(t)
+            both.append(c * torch.exp2(b.double() - 127)[..., None])
+            assert torch.equal(out.cpu().double(), both[-1])
+        held.append(tuple(both))
+    assert int(status.item()) == 0
+    q = rows_of(requests, heads, dim, 3)
+    for plan in (None, (1, 2, 1, 2, 1, 2, 8)):
+        out, told = attend(native, {"k_cache": codes[0], "table": table}, requests, q, 0, 0, dim ** -0.5, plan=plan, caches=caches)
+        assert told == 0
+        check_attention({"k_cache": codes[0], "held": held}, requests, q, out, 0, 0, dim ** -0.5)
