@@ -371,7 +371,7 @@ struct WarpRing {
 // bits down to 2^-11 of the row's largest element and what is smaller to within 2^-18 of it; the tensor core sums them
 // to within 6e-8 of the sum of magnitudes.  Values go in as half-precision numbers, 16 of their elements on the side of
 // 16, so an output comes out transposed too.  One sequence of 32768 keys, 32 heads on 8: 25.9 us, where 16 rows a
-// product took 28.1; eight of 2048: 16.0 and 17.8 (21.5 and 13.9 since the cuts and launches below).  32 sequences of
+// product took 28.1; eight of 2048: 16.0 and 17.8 (21.6 and 14.3 since the cuts and launches below).  32 sequences of
 // up to 8192 keys: 61 to 65 us, 0.70 of the copy peak; instructions issue in 47 % of the cycles, three warps a scheduler
 // (registers and rings allow 12 an SM) wait for one another's latencies, not for memory.
 struct RowQueries {

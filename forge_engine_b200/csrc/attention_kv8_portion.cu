@@ -22,7 +22,7 @@
 // values: 7,700 cycles a tile, all of it the staging warps.  20 warps, of 96 and of 120 registers, were slower too.
 //
 // A tile takes 4,600 to 5,000 cycles (2.6 to 3.2 us), a block about 9 us beside its tiles (row tile, pages, first keys and
-// queries one after the other, the last products and stores): 2,048 tokens from the start 68 us, 509 behind 32,259
+// queries one after the other, the last products and stores): 2,048 tokens from the start 69 us, 509 behind 32,259
 // keys 435.  The tensor core works in 26 to 38 % of the cycles, the exponentials' unit in 27 to 39 %, instructions issue in
 // 49 to 55 %: what bounds a tile is the chain of a softmax warp's half (scores out, maximum, exponentials, weights
 // back), of which a scheduler holds two beside the staging warps; registers leave no room for a third.
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_portion_kernel(Kv8Attenti
   if (warp >= SOFTMAX_WARPS && warp < MMA_WARP) {
     // ---- staging ----
     const int* table = p.block_table + (size_t)at.entry * p.max_pages;
-    // Piece j of this lane is 16 bytes of one of the warp's rows, unit w + 8 j; the lanes of a unit lie so that eight
+    // Piece j of this lane is 16 bytes of one of the warp's rows, unit w + 6 j; the lanes of a unit lie so that eight
     // neighbours store their 32 bytes of bfloat16 without meeting in a bank.  A lane looks after one of the warp's
     // rows - its page, its place and its scales - and the others ask it.
     constexpr int UNIT_ROWS = 32 / CHUNKS;

@@ -151,7 +151,7 @@ constexpr int WRITE_ROUNDS = 64;                 // heads a group of lanes takes
 // that rotate together.  With R rotated dimensions pair i < R/2 is (i, i + R/2); the others pair up
 // (R + i', R + (D - R)/2 + i') and stay as they are.  R is a multiple of 2E, so E pairs are two stretches of E elements.
 // E = 8 where rows and R allow 16-byte loads of bfloat16, else 4.  Queries are not measured for a scale, values not
-// normalised.  4,096 tokens of 32 + 16 heads of 128: 27.5 us, 0.53 of the copy peak, instructions issued in most cycles
+// normalised.  4,096 tokens of 32 + 16 heads of 128: 27.2 us, 0.53 of the copy peak, instructions issued in most cycles
 // (34.6 with E = 4; 24.2 when keys' codes were those of 32-bit arithmetic: 1.7 for the span's second end, the rest for heads
 // taken again; with that inside the loop, where its registers count, 34.6).  64 tokens in 32 bits 5.0, one 3.4, most
 // of it the launch and the first loads.  Seven blocks an SM: 27.5 us, eight, with 40 bytes of spills, 28.3, six 28.5.

@@ -2097,13 +2097,14 @@ def _kv8_tiles(start: int, first: int, last: int, window: int, keep_first: int, 
     return kept + -(-(start + last + 1) // tile) - low
 
 
-# What a block of the attention over an 8-bit cache costs on a B200, in microseconds, fitted to measured calls: (blocks the
-# GPU holds at once, a key tile of a block where they share their SMs as cut entries do, the same where all SMs are full, a
-# block beside its tiles, joining the pieces of cut entries, of that each piece of the longest).  Up to 8 rows: 8 requests of
-# 2,048 keys 13.8 us with 4 tiles a block (320 blocks), 16.5 with 2 (576: a second round), 15.8 with 8, 23.5 uncut; 100,000
+# What a block of the attention over an 8-bit cache costs on a B200, in microseconds, fitted to measured calls, those
+# of single tokens and of tcgen05 portions with heads of 128, and used for every head size, though large heads' blocks are fewer
+# at once (256: one an SM) and slower: (blocks the GPU holds at once, a key tile of a block where they share their SMs as cut
+# entries do, the same where all SMs are full, a block beside its tiles, joining the pieces of cut entries, of that each piece of
+# the longest).  Up to 8 rows: 8 requests of 2,048 keys 13.8 us with 4 tiles a block (320 blocks), 16.5 with 2 (576: a second round), 15.8 with 8, 23.5 uncut; 100,000
 # keys of one 45.6 with 24, 65.7 with 4.  9 to 16 rows: 48 requests in a window of 4,096 84 uncut, 116 with 4.  Portions:
-# 509 tokens behind 32,259 keys 421 us with 64 tiles a block (256 blocks), 433 with 128 (128), 538 with 86 (192: the second
-# round is half empty), 824 uncut.
+# 509 tokens behind 32,259 keys 422 us with 64 tiles a block (256 blocks), 435 with 128 (128), 537 with 86 (192: the second
+# round is half empty), 820 uncut; of the first two, 3 % apart, the cost prefers the second.
 _KV8_FEW = (444, 1.3, 2.6, 3.3, 4.2, 0.04)
 _KV8_SINGLE = (444, 1.7, 2.4, 6.6, 6.8, 0.02)
 _KV8_PORTION = (148, 3.2, 3.2, 9.0, 8.0, 0.0)
